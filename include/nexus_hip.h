@@ -33,6 +33,10 @@
  *   TurboQuant paged KV (head_dim 128): codes4 [num_blocks][hkv][16][32] u8,
  *     codes3 [num_blocks][hkv][16][24] u8, norms [num_blocks][hkv][16] fp16;
  *     58 bytes per vector (see nx_tq_encode).
+ *   int4-g32 paged KV (head_dim 64, 128, 256): pools [num_blocks][hkv][9 *
+ *     head_dim] bytes; a page of one kv head holds 16 tokens x head_dim codes
+ *     of 4 bits and a fp16 scale per token and 32 dimensions, value =
+ *     (code - 8) * scale; 9/16 byte per value (see nx_kv_append_int4).
  */
 #ifndef NEXUS_HIP_H
 #define NEXUS_HIP_H
@@ -226,6 +230,73 @@ nx_status nx_attn_decode_paged_tq(nx_ctx* ctx, nx_buf q_f32, nx_buf kc4, nx_buf 
                                   nx_buf vc4, nx_buf vc3, nx_buf vn, nx_buf ksigns, nx_buf vsigns,
                                   nx_buf block_table, nx_buf ctx_lens_i32, nx_buf out_f16,
                                   int batch, int hq, int hkv, int max_blocks, int num_blocks);
+/* ---- int4-g32 KV pages.  For a cache of 9/32 of fp16 pages' size with heads
+ * of 64, 128 or 256.  These calls check lengths, positions and block tables
+ * in their kernels: they do not wait for the device and may be captured into
+ * a token batch; what a sequence out of range gets is said at each call.
+ *
+ * Append `tokens` rows per sequence, k and v fp32 [batch][tokens][hkv]
+ * [head_dim]: row i of sequence b goes to position positions[b] + i through
+ * the block table (one row in decode, a prompt's in prefill).  Per token and
+ * group of 32 dimensions: scale = fp16(amax / 7), at most 65504; code =
+ * clamp(roundf(x / scale), -8, 7) + 8, quotients rounded to fp32 (a scale of
+ * 0 has code 8); a group that holds a NaN or an infinity gets a NaN scale and
+ * reads back as NaN.  Rows of a sequence that would begin below 0 or end
+ * beyond max_blocks * 16 are not written, nor are rows whose table entry lies
+ * outside [0, num_blocks).  tokens beyond max_blocks * 16: NX_ERR_CAPACITY.
+ * Two sequences must not write to one page. */
+nx_status nx_kv_append_int4(nx_ctx* ctx, nx_buf k_f32, nx_buf v_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
+                            nx_buf positions_i32, int batch, int tokens, int hkv, int head_dim, int max_blocks,
+                            int num_blocks);
+/* The values that pages hold, back as fp32 rows [batch][tokens][hkv]
+ * [head_dim] from position positions[b] on (the gather of
+ * PagedKVCache::get_vectors, kv/paged_attention.cpp:161-230).  Rows that
+ * nx_kv_append_int4 would not write are NaN. */
+nx_status nx_kv_read_int4(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block_table, nx_buf positions_i32, nx_buf k_f32,
+                          nx_buf v_f32, int batch, int tokens, int hkv, int head_dim, int max_blocks, int num_blocks);
+/* Decode attention over int4-g32 pages: out[b][h] = softmax(q.K^T /
+ * sqrt(head_dim)) V over positions [0, ctx_lens[b]), out fp16
+ * [batch][hq][head_dim], zeros for a length of 0.  hq / hkv up to 64.
+ * weights_f32 (0: none) is [batch][hkv][max_blocks * 16]: every position's
+ * softmax weight, summed over the query heads of its kv head, is added to it;
+ * slots at ctx_lens[b] and above are left as they are.  A sequence whose
+ * length exceeds max_blocks * 16 (or is negative), or whose table names a block
+ * outside [0, num_blocks) for one of its pages, gets NaN output rows and its
+ * weights stay as they are. */
+nx_status nx_attn_decode_paged_int4(nx_ctx* ctx, nx_buf q_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
+                                    nx_buf ctx_lens_i32, nx_buf out_f16, nx_buf weights_f32, int batch, int hq, int hkv,
+                                    int head_dim, int max_blocks, int num_blocks);
+/* The same over fp16 pages, weights required: nx_attn_decode_paged_f16 (any
+ * hq / hkv up to 64) that also accumulates the weights. */
+nx_status nx_attn_decode_paged_f16_acc(nx_ctx* ctx, nx_buf q_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
+                                       nx_buf ctx_lens_i32, nx_buf out_f16, nx_buf weights_f32, int batch, int hq, int hkv,
+                                       int head_dim, int max_blocks, int num_blocks);
+/* Eviction by accumulated weight: every sequence with more than `keep` tokens
+ * cached is cut to `keep`, each kv head by its own weights.  seen[b] is the
+ * number of tokens the sequence has had so far (at least ctx_lens[b]), and a
+ * tag in tags_i32 [batch][hkv][max_blocks * 16] is the position of a slot's
+ * token in the sequence plus 1, or 0 for a token appended since the last call
+ * (slot s then holds position seen[b] - ctx_lens[b] + s): zeros to begin with,
+ * as nx_alloc gives them.  Of a kv head's slots stay first those whose
+ * position is seen[b] - recent or later, then those of larger weight, the
+ * lower slot among equals (NaN is below every number).  Tokens that stay move
+ * from slots >= keep into the free ones below, the i-th to the i-th; the slots
+ * are then [0, keep) in no particular order, which attention does not mind
+ * (keys carry their rotation).  weights_out and tags_out get the slots' weights
+ * and tags, zeros from the new length on; lens_out[b] the new length, the next
+ * token's slot; pages past it are free.  Each of the three may be its input.  A
+ * sequence of at most `keep` tokens moves nothing.  One whose length is out of
+ * range or above seen[b], or whose table names a block outside the pool, gets
+ * lens_out[b] = -1 and stays as it is.  Sequences must not share pages. */
+nx_status nx_kv_evict_f16(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block_table, nx_buf ctx_lens_i32, nx_buf seen_i32,
+                          nx_buf weights_f32, nx_buf tags_i32, nx_buf lens_out_i32, nx_buf weights_out_f32,
+                          nx_buf tags_out_i32, int batch, int hkv, int head_dim, int max_blocks, int num_blocks, int keep,
+                          int recent);
+/* The same over int4-g32 pages. */
+nx_status nx_kv_evict_int4(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block_table, nx_buf ctx_lens_i32, nx_buf seen_i32,
+                           nx_buf weights_f32, nx_buf tags_i32, nx_buf lens_out_i32, nx_buf weights_out_f32,
+                           nx_buf tags_out_i32, int batch, int hkv, int head_dim, int max_blocks, int num_blocks, int keep,
+                           int recent);
 /* MoE routing: softmax over E logits fp32 [batch][E], top-k by probability
  * (ties: lower id), renormalized weights.  hybrid_model.cpp:1656-1694.
  * E <= 256, k <= min(16, E), batch <= 64. */

@@ -8,6 +8,7 @@
 #include <chrono>
 #include <cmath>
 #include <cstring>
+#include <new>
 #include <random>
 
 #include "nx_common.h"
@@ -167,6 +168,17 @@ extern "C" {
 // Not part of the interface: lets a test take away the device's memory.
 void nx_limit_allocations(nx_ctx* ctx, size_t bytes) { ctx->alloc_limit = bytes; }
 
+// Not part of the interface: a context without a device, whose buffers (ids
+// 1 .. n of the given sizes) are numbers alone, to test what calls refuse
+// before they reach a device.
+nx_ctx* nx_deviceless(const size_t* bytes, int n) {
+    nx_ctx* ctx = new (std::nothrow) nx_ctx();
+    if (!ctx) return nullptr;
+    ctx->device = -1;
+    for (int i = 0; i < n; ++i) ctx->bufs[(uint64_t)i + 1] = bytes[i];
+    return ctx;
+}
+
 // ---------------------------------------------------------------- lifecycle --
 int nx_has_gpu(void) {
     int n = 0;
@@ -224,6 +236,10 @@ nx_status nx_init(nx_ctx** out, int device) {
 
 nx_status nx_destroy(nx_ctx* ctx) {
     if (!ctx) return NX_ERR_INVALID;
+    if (ctx->device < 0) {  // nx_deviceless
+        delete ctx;
+        return NX_OK;
+    }
     (void)hipSetDevice(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
     nx::detach_models(ctx);
@@ -238,6 +254,7 @@ nx_status nx_destroy(nx_ctx* ctx) {
     if (ctx->attn_chk_host) (void)hipHostFree(ctx->attn_chk_host);
     if (ctx->smp_ws) (void)hipFree(ctx->smp_ws);
     if (ctx->gemv_ws) (void)hipFree(ctx->gemv_ws);
+    if (ctx->kvc_ws) (void)hipFree(ctx->kvc_ws);
     for (void* p : ctx->outgrown) (void)hipFree(p);
     (void)hipEventDestroy(ctx->ev0);
     (void)hipEventDestroy(ctx->ev1);
@@ -1303,6 +1320,7 @@ nx_status nx_reserve_workspace(nx_ctx* ctx, int batch, int max_ffn, int vocab, i
         if (max_ctx > nx::attn_max_ctx()) return fail(ctx, NX_ERR_UNSUPPORTED, "max_ctx above the attention limit");
         s = ensure_attn_ws(ctx, nx::attn_workspace_bytes(batch, n_heads, n_kv_heads, head_dim, max_ctx));
         if (s == NX_OK) s = ensure_attn_counts(ctx, nx::attn_count_words(batch, n_kv_heads));
+        if (s == NX_OK) s = nx::kvc_reserve(ctx, batch, n_heads, n_kv_heads, head_dim, max_ctx);
         chk = nx::attn_check_words(batch, (max_ctx + nx::kPage - 1) / nx::kPage);
     }
     if (s == NX_OK) s = ensure_attn_chk(ctx, chk);  // (the routed experts' plan check as well)

@@ -50,6 +50,9 @@ struct nx_ctx {
     // capture, one launch streams all of K) and of GEMMs; grow-only
     float* gemv_ws = nullptr;
     size_t gemv_ws_floats = 0;
+    // workspace of the compact cache's attention and eviction (grow-only)
+    void* kvc_ws = nullptr;
+    size_t kvc_ws_bytes = 0;
     // workspaces outgrown while a token batch was captured, which its
     // launches still name: freed once the batch has run
     std::vector<void*> outgrown;
@@ -92,6 +95,9 @@ template <class T>
 hipError_t dev_malloc(nx_ctx* ctx, T** p, size_t bytes) {
     return dev_malloc(ctx, reinterpret_cast<void**>(p), bytes);
 }
+
+// The compact cache's part of nx_reserve_workspace.
+nx_status kvc_reserve(nx_ctx* ctx, int batch, int hq, int hkv, int hd, int max_ctx);
 
 // Size of a buffer of the context, 0 if it is not one.
 inline size_t buf_size(const nx_ctx* ctx, nx_buf b) {

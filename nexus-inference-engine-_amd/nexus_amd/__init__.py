@@ -126,6 +126,12 @@ _SIGS = {
     "nx_kv_append_f16": (_I, [_P, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I]),
     "nx_attn_decode_paged_f16": (_I, [_P, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I]),
     "nx_attn_decode_paged_f16_noalloc": (_I, [_P, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I]),
+    "nx_kv_append_int4": (_I, [_P, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I]),
+    "nx_kv_read_int4": (_I, [_P, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I]),
+    "nx_attn_decode_paged_int4": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I]),
+    "nx_attn_decode_paged_f16_acc": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I]),
+    "nx_kv_evict_f16": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I, _I]),
+    "nx_kv_evict_int4": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I, _I]),
     "nx_tq_codebooks": (_I, [_P, _P, _P, _P]),
     "nx_tq_encode": (_I, [_P, _B, _B, _B, _B, _B, _I]),
     "nx_tq_append": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I]),
@@ -324,6 +330,39 @@ class Context:
     def gemv_f32(self, x, wq, sc, y, N, K, batch=1, accumulate=False):
         self.check(self.L.nx_gemv_int4_g32_f32(self.h, x, wq, sc, y, N, K, batch, int(accumulate)),
                    "nx_gemv_int4_g32_f32")
+
+    # the compact KV cache (include/nexus_hip.h); buffers are handles
+    def kv_append_int4(self, k, v, kpool, vpool, table, positions, batch, tokens, hkv, head_dim, max_blocks, num_blocks):
+        self.check(self.L.nx_kv_append_int4(self.h, k, v, kpool, vpool, table, positions, batch, tokens, hkv, head_dim,
+                                            max_blocks, num_blocks), "nx_kv_append_int4")
+
+    def kv_read_int4(self, kpool, vpool, table, positions, k, v, batch, tokens, hkv, head_dim, max_blocks, num_blocks):
+        self.check(self.L.nx_kv_read_int4(self.h, kpool, vpool, table, positions, k, v, batch, tokens, hkv, head_dim,
+                                          max_blocks, num_blocks), "nx_kv_read_int4")
+
+    def attn_decode_paged_int4(self, q, kpool, vpool, table, ctx_lens, out, weights, batch, hq, hkv, head_dim,
+                               max_blocks, num_blocks):
+        """weights 0: none are accumulated."""
+        self.check(self.L.nx_attn_decode_paged_int4(self.h, q, kpool, vpool, table, ctx_lens, out, weights, batch, hq,
+                                                    hkv, head_dim, max_blocks, num_blocks), "nx_attn_decode_paged_int4")
+
+    def attn_decode_paged_f16_acc(self, q, kpool, vpool, table, ctx_lens, out, weights, batch, hq, hkv, head_dim,
+                                  max_blocks, num_blocks):
+        self.check(self.L.nx_attn_decode_paged_f16_acc(self.h, q, kpool, vpool, table, ctx_lens, out, weights, batch,
+                                                       hq, hkv, head_dim, max_blocks, num_blocks),
+                   "nx_attn_decode_paged_f16_acc")
+
+    def kv_evict_f16(self, kpool, vpool, table, ctx_lens, seen, weights, tags, lens_out, weights_out, tags_out, batch,
+                     hkv, head_dim, max_blocks, num_blocks, keep, recent):
+        self.check(self.L.nx_kv_evict_f16(self.h, kpool, vpool, table, ctx_lens, seen, weights, tags, lens_out,
+                                          weights_out, tags_out, batch, hkv, head_dim, max_blocks, num_blocks, keep,
+                                          recent), "nx_kv_evict_f16")
+
+    def kv_evict_int4(self, kpool, vpool, table, ctx_lens, seen, weights, tags, lens_out, weights_out, tags_out, batch,
+                      hkv, head_dim, max_blocks, num_blocks, keep, recent):
+        self.check(self.L.nx_kv_evict_int4(self.h, kpool, vpool, table, ctx_lens, seen, weights, tags, lens_out,
+                                           weights_out, tags_out, batch, hkv, head_dim, max_blocks, num_blocks, keep,
+                                           recent), "nx_kv_evict_int4")
 
 
 class Model:
