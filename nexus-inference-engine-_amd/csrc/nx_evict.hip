@@ -8,11 +8,10 @@
 // destinations below, and no copy can overtake another.
 //
 // k_pick, one block per (sequence, kv head): a radix selection over 32-bit
-// keys (11, 11 and 10 bits) finds the keep-th largest, ballots number the
-// equal ones, the free slots and the tokens that move in slot order, and the
-// weights and tags are written.  k_move, one wavefront per destination page:
-// K vectors as they are; V, whose pages are dimension-major, by rewriting the
-// page's words, each of which one lane owns.
+// keys (11, 11 and 10 bits), which stay in LDS, finds the keep-th largest; ballots number the equal ones, the free slots and the
+// tokens that move in slot order.  k_move, one wavefront per destination page:
+// weights and tags; K vectors as they are; V, whose pages are dimension-major,
+// by rewriting the page's words, each of which one lane owns.
 #include <algorithm>
 
 #include "nx_kvc.h"
@@ -23,67 +22,108 @@ namespace kvc {
 namespace {
 
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / kWave;
-constexpr int kBins = 2048;
+constexpr int kBins = 2048, kListed = 2048;
+constexpr int kKeyPad = 8 * kWave;  // keys past a row's that a wavefront may read
+constexpr int kLdsSlots = 32768;  // slots whose keys a block holds in LDS
 
-// The words a (sequence, kv head) has in the workspace: keys, then where each
-// kept slot's token comes from (-1: it stays), then the tokens that move.
-struct Row {
-    uint32_t* keys;
-    int32_t *src, *from;
-};
 __host__ __device__ inline int kept_slots(int max_blocks, int keep) {
     const int cap = max_blocks * kPage;
     return keep < cap ? (keep + kPage - 1) / kPage * kPage : cap;
 }
-__device__ inline Row row_of(const EvictArgs& a, int b, int h) {
-    const size_t cap = (size_t)a.max_blocks * kPage, ks = kept_slots(a.max_blocks, a.keep);
-    uint32_t* p = a.ws + ((size_t)b * a.hkv + h) * (cap + 2 * ks);
-    return {p, reinterpret_cast<int32_t*>(p + cap), reinterpret_cast<int32_t*>(p + cap + ks)};
-}
-__device__ inline int32_t* new_lens(const EvictArgs& a) {
-    const size_t cap = (size_t)a.max_blocks * kPage, ks = kept_slots(a.max_blocks, a.keep);
-    return reinterpret_cast<int32_t*>(a.ws + (size_t)a.batch * a.hkv * (cap + 2 * ks));
+// Slots whose keys go through memory: longer rows than LDS holds.
+__host__ __device__ inline size_t stored_keys(int max_blocks) {
+    const size_t cap = (size_t)max_blocks * kPage;
+    return cap > (size_t)kLdsSlots ? (cap + kPickThreads - 1) / kPickThreads * kPickThreads + 8 * kWave : 0;
 }
 
-// Order of weights as unsigned numbers: NaN below every other, -0 as 0.
+// What k_pick leaves for k_move.  Of a sequence: its new length (-1: refused),
+// whether it was cut, and what a slot's number lacks to the tag of a token
+// appended since the last call.  Of a (sequence, kv head) that is cut: a bit
+// for each slot that stays, 64 to a word; for each word how many slots below
+// keep came free before it; and the slots of the tokens that move, in order.
+struct Seq {
+    int len, cut, ahead;
+};
+constexpr int kSeqWords = 4;
+__device__ inline Seq* seq_of(const EvictArgs& a, int b) { return reinterpret_cast<Seq*>(a.ws + (size_t)b * kSeqWords); }
+__host__ __device__ inline size_t bit_words(int max_blocks) { return ((size_t)max_blocks * kPage + kWave - 1) / kWave; }
+__host__ __device__ inline size_t row_words(int max_blocks, int keep) {
+    return (3 * bit_words(max_blocks) + kept_slots(max_blocks, keep) + stored_keys(max_blocks) + 1) / 2 * 2;
+}
+struct Row {
+    unsigned long long* stays;
+    int32_t *free_before, *from;
+    uint32_t* keys;
+};
+__device__ inline Row row_of(const EvictArgs& a, int b, int h) {
+    const size_t nw = bit_words(a.max_blocks);
+    uint32_t* p = a.ws + (size_t)a.batch * kSeqWords + ((size_t)b * a.hkv + h) * row_words(a.max_blocks, a.keep);
+    int32_t* q = reinterpret_cast<int32_t*>(p + 2 * nw);
+    return {reinterpret_cast<unsigned long long*>(p), q, q + nw, p + 3 * nw + kept_slots(a.max_blocks, a.keep)};
+}
+
+// Order of weights as unsigned numbers: NaN below every other, -0 as 0; no
+// weight has key 0, which stands for no token.
 __device__ inline uint32_t weight_key(float w) {
-    if (w != w) return 0u;
+    if (w != w) return 1u;
     const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sums of v over the block in thread order, and their total.
-__device__ inline int block_scan(int v, int* lds, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const int y = __shfl_up(x, o, kWave);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) lds[wave] = x;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int w = 0; w < kPickWaves; ++w) {
-        before += w < wave ? lds[w] : 0;
-        total += lds[w];
-    }
-    return before + x - v;
+// base + the bits of v below this lane.
+__device__ inline int below_lane(unsigned long long v, int base) {
+    return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(v >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)v, (unsigned)base));
 }
 
+template <int CTRL, int ROWS = 0xF>
+__device__ inline int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+// Inclusive sums over the 16 lanes of a row.
+__device__ inline int row_scan(int v) {
+    v = dpp_add<0x111>(v);  // row_shr:1, 2, 4, 8
+    v = dpp_add<0x112>(v);
+    v = dpp_add<0x114>(v);
+    return dpp_add<0x118>(v);
+}
+// Inclusive sums over the wavefront's lanes.
+__device__ inline int wave_scan(int v) { return dpp_add<kRowBcast31, 0xC>(dpp_add<kRowBcast15, 0xA>(row_scan(v))); }
+// Exclusive sums over the block in thread order of two numbers, and their totals.
+__device__ inline int2 block_scan(int2 v, int2* lds, int2& total) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = wave_scan(v.x), y = wave_scan(v.y);
+    __syncthreads();
+    if (lane == kWave - 1) lds[wave] = make_int2(x, y);
+    __syncthreads();
+    static_assert(kPickWaves == 16, "one row of lanes holds the wavefronts' sums");
+    const int2 w = lds[lane & 15];
+    const int wx = row_scan(w.x), wy = row_scan(w.y);
+    total = make_int2(__builtin_amdgcn_readlane(wx, 15), __builtin_amdgcn_readlane(wy, 15));
+    const int2 before = wave > 0 ? make_int2(__builtin_amdgcn_readlane(wx, wave - 1), __builtin_amdgcn_readlane(wy, wave - 1)) : make_int2(0, 0);
+    return make_int2(before.x + x - v.x, before.y + y - v.y);
+}
+
+// SLOTS: the longest row whose keys stay in LDS; 0: they go through memory.
+// A block is one compute unit's work and bound by its instructions and, in the
+// first loop, by what one compute unit can request; a row's slots are passed
+// three times: keys and their top bits are counted, the keys of the bin that
+// holds the keep-th are listed, and the keys are compared with the keep-th.
+// 32768 slots of 8 kv heads: 22 us, 4352: 9 us.
+template <int SLOTS>
 __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
-    __shared__ uint32_t hist[kBins];
-    __shared__ int sums[kPickWaves], found_bin, found_left;
+    // two counters per bin, by lane: weights crowd into few bins
+    __shared__ uint2 hist[kBins];
+    __shared__ uint32_t lds_keys[SLOTS > 0 ? SLOTS + kKeyPad : 1], list[kListed];
+    __shared__ int2 sums[kPickWaves];
+    __shared__ int found_bin, found_left, found_all, listed;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int cap = a.max_blocks * kPage, keep = a.keep, L = a.lens_in[b], N = a.seen[b], ks = kept_slots(a.max_blocks, keep);
+    const int cap = a.max_blocks * kPage, keep = a.keep, L = a.lens_in[b], N = a.seen[b];
     const Row r = row_of(a, b, h);
     const size_t at = ((size_t)b * a.hkv + h) * cap;
     const float* w_in = a.weights_in + at;
     const int32_t* t_in = a.tags_in + at;
-    float* w_out = a.weights_out + at;
-    int32_t* t_out = a.tags_out + at;
+    for (int i = tid; i < kBins; i += kPickThreads) hist[i] = make_uint2(0u, 0u);
+    if (tid == 0) listed = 0;
     bool bad = L < 0 || L > cap || N < L;
     if (!bad)
         for (int p = tid; p < (L + kPage - 1) / kPage; p += kPickThreads) {
@@ -91,186 +131,398 @@ __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
             bad = bad || blk < 0 || blk >= a.num_blocks;
         }
     bad = __syncthreads_or(bad);
-    if (tid == 0 && h == 0) new_lens(a)[b] = bad ? -1 : min(L, keep);
-    // a token's position + 1: its tag, or its place among the tokens
-    // appended since the last call
-    auto tag_of = [&](int s) {
-        const int t = t_in[s];
-        return t > 0 ? t : N - L + s + 1;
+    if (tid == 0 && h == 0) *seq_of(a, b) = {bad ? -1 : min(L, keep), !bad && L > keep, N - L + 1};
+    if (bad || L <= keep) return;
+    uint32_t* keys;
+    if constexpr (SLOTS > 0)
+        keys = lds_keys;
+    else
+        keys = r.keys;
+    // a wavefront takes a run of slots, lane l of step u slot s0 + 64 u + l
+    // (no thread uses a key that another wrote); slots past the row's last
+    // token have key 0, kKeyPad more may be read
+    const int steps = (L + kPickThreads - 1) / kPickThreads, s0 = wave * steps * kWave, s1 = min(L, s0 + steps * kWave);
+    const int mine_n = (max(s1 - s0, 0) + kWave - 1) / kWave;  // steps of this wavefront
+    // f(step, key) over n steps from slot `first` on, eight keys requested together
+    auto over = [&](int first, int n, auto&& f) {
+        for (int u0 = 0; u0 < n; u0 += 8) {
+            const uint32_t* p = keys + first + u0 * kWave + lane;
+            uint32_t k[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) k[j] = p[j * kWave];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (u0 + j < n) f(u0 + j, k[j]);
+        }
     };
-    if (bad || L <= keep) {
-        for (int s = tid; s < ks; s += kPickThreads) r.src[s] = -1;
-        if (bad) return;
-        for (int s = tid; s < cap; s += kPickThreads) {
-            const float w = s < L ? w_in[s] : 0.0f;
-            const int t = s < L ? tag_of(s) : 0;
-            w_out[s] = w;
-            t_out[s] = t;
+    // ---- the keep-th largest key.  Recent tokens have the largest and are
+    // counted apart.
+    uint32_t* count = reinterpret_cast<uint32_t*>(hist) + (lane & 1);
+    int recents = 0;
+    for (int u0 = 0; u0 < mine_n; u0 += 8) {
+        float w[8];
+        int t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int s = min(s0 + (u0 + j) * kWave + lane, s1 - 1);
+            w[j] = w_in[s];
+            t[j] = t_in[s];
         }
-        return;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (u0 + j >= mine_n) break;
+            const int s = s0 + (u0 + j) * kWave + lane, tag = t[j] > 0 ? t[j] : N - L + s + 1;
+            const bool in = s < s1, recent = in && tag > N - a.recent;
+            const uint32_t key = recent ? 0xFFFFFFFFu : in ? weight_key(w[j]) : 0u;
+            keys[s] = key;
+            recents += recent;
+            if (key - 1u < 0xFFFFFFFEu) atomicAdd(count + 2 * (key >> 21), 1u);
+        }
     }
-    // a wavefront takes a run of slots, 64 at a time
-    const int run = (L + kPickThreads - 1) / kPickThreads * kWave, s0 = wave * run, s1 = min(L, s0 + run);
-    // ---- the keep-th largest key
-    uint32_t prefix = 0u, mask = 0u;
-    int left = keep;
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-        for (int i = tid; i < kBins; i += kPickThreads) hist[i] = 0u;
-        __syncthreads();
-        for (int s = s0 + lane; s < s1; s += kWave) {
-            uint32_t key;
-            if (pass == 0) {
-                key = tag_of(s) > N - a.recent ? 0xFFFFFFFFu : weight_key(w_in[s]);
-                r.keys[s] = key;
-            } else {
-                key = r.keys[s];
-            }
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
-        }
-        __syncthreads();
-        // thread i: bins 2047 - 2 i and 2046 - 2 i, the largest keys first
-        const int hi = (int)hist[kBins - 1 - 2 * tid], lo = (int)hist[kBins - 2 - 2 * tid];
-        int total;
-        const int before = block_scan(hi + lo, sums, total);
+    __syncthreads();
+    int2 total;
+    uint32_t prefix = 0u;
+    int left = 0, all = 0;
+    // The bin of the counts in which the left-th largest lies: thread i adds up
+    // bins 2047 - 2 i and 2046 - 2 i, the largest keys first.
+    auto find = [&](int shift, bool first_pass) {
+        const uint2 x = hist[kBins - 1 - 2 * tid], y = hist[kBins - 2 - 2 * tid];
+        const int hi = (int)(x.x + x.y), lo = (int)(y.x + y.y);
+        const int before = block_scan(make_int2(hi + lo, recents), sums, total).x;
+        if (first_pass) left = keep - total.y;
         if (before < left && left <= before + hi + lo) {
             const bool first = left <= before + hi;
             found_bin = first ? kBins - 1 - 2 * tid : kBins - 2 - 2 * tid;
             found_left = left - before - (first ? 0 : hi);
+            found_all = first ? hi : lo;
         }
         __syncthreads();
+        if (left <= 0) return;
         prefix |= (uint32_t)found_bin << shift;
-        mask |= (uint32_t)(bins - 1) << shift;
         left = found_left;
-        __syncthreads();
-    }
-    // ---- keys above the prefix stay, of the equal ones the `left` lowest slots
-    int total, equal = 0;
-    for (int s = s0 + lane; s < s1; s += kWave) equal += r.keys[s] == prefix;
-    // (a wavefront's lanes in one sum: the scan is by thread, its run by wavefront)
-    for (int o = 1; o < kWave; o <<= 1) equal += __shfl_xor(equal, o, kWave);
-    const int eq0 = __shfl(block_scan(lane == 0 ? equal : 0, sums, total), 0, kWave);
-    int holes0 = 0, moves0 = 0;
-    for (int write = 0; write < 2; ++write) {
-        int eq = eq0, holes = holes0, moves = moves0;
-        for (int s = s0 + lane; s - lane < s1; s += kWave) {
-            const uint32_t key = s < s1 ? r.keys[s] : 0u;
-            const unsigned long long below = (1ull << lane) - 1ull;
-            const unsigned long long same = __ballot(s < s1 && key == prefix);
-            const bool kept = s < s1 && (key > prefix || (key == prefix && eq + __popcll(same & below) < left));
-            const unsigned long long hole = __ballot(s < s1 && s < keep && !kept), move = __ballot(kept && s >= keep);
-            if (write) {
-                const bool mine = hole >> lane & 1ull;
-                if (s < min(s1, keep)) r.src[s] = mine ? holes + __popcll(hole & below) : -1;
-                if (move >> lane & 1ull) r.from[moves + __popcll(move & below)] = s;
-            }
-            eq += __popcll(same);
-            holes += __popcll(hole);
-            moves += __popcll(move);
+        all = found_all;
+    };
+    find(21, true);
+    if (left <= 0) {
+        prefix = 0xFFFFFFFFu;
+        left = keep;
+        all = total.y;
+    } else {
+        // the bin's keys in a list, if they are few, so that the other bits
+        // take no more passes over the row
+        uint32_t base = max(prefix, 1u), span = prefix + (1u << 21) - base;
+        const bool few = all <= kListed;
+        if (few)
+            over(s0, mine_n, [&](int, uint32_t key) {
+                if (key - base < span) list[atomicAdd(&listed, 1)] = key;
+            });
+        for (int shift = 10; shift >= 0; shift -= 10) {
+            const uint32_t last = shift ? 2047u : 1023u;
+            for (int i = tid; i < kBins; i += kPickThreads) hist[i] = make_uint2(0u, 0u);
+            __syncthreads();
+            auto add = [&](int, uint32_t key) {
+                if (key - base < span) atomicAdd(count + 2 * ((key >> shift) & last), 1u);
+            };
+            if (few)
+                for (int i = tid; i < listed; i += kPickThreads) add(0, list[i]);
+            else
+                over(s0, mine_n, add);
+            __syncthreads();
+            find(shift, false);
+            base = max(prefix, 1u);
+            span = prefix + (1u << shift) - base;
+            __syncthreads();
         }
-        if (!write) {
-            const int x = block_scan(lane == 0 ? holes : 0, sums, total), y = block_scan(lane == 0 ? moves : 0, sums, total);
-            holes0 = __shfl(x, 0, kWave);
-            moves0 = __shfl(y, 0, kWave);
-        }
     }
-    __syncthreads();
-    // ---- the kept slots' weights and tags; then nothing beyond them
-    for (int s = tid; s < ks; s += kPickThreads) {
-        if (s >= keep) {
-            r.src[s] = -1;
-            continue;
-        }
-        const int i = r.src[s], m = i < 0 ? s : r.from[i];
-        if (i >= 0) r.src[s] = m;
-        const float w = w_in[m];
-        const int t = tag_of(m);
-        w_out[s] = w;
-        t_out[s] = t;
+    // ---- keys above the prefix stay, of the `all` equal ones the `left`
+    // lowest slots.  Each step's comparison is a word of 64 bits, which lane u
+    // keeps for step u of a round; counts and running sums over the steps are
+    // then one vector operation (the scalar unit, which all of the block's
+    // wavefronts share, took longer for them step by step).
+    typedef unsigned long long Bits;
+    const bool ties = all != left;
+    const int rounds = (steps + kWave - 1) / kWave;
+    auto bits_of = [&](int round, auto&& f) {
+        uint32_t lo = 0u, hi = 0u;
+        over(s0 + round * kWave * kWave, min(mine_n - round * kWave, kWave), [&](int u, uint32_t key) {
+            const Bits v = __ballot(f(u, key));
+            lo = lane == u ? (uint32_t)v : lo;
+            hi = lane == u ? (uint32_t)(v >> 32) : hi;
+        });
+        return (Bits)hi << 32 | lo;
+    };
+    auto lane_bits = [&](Bits v, int u) {
+        return (Bits)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), u) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, u);
+    };
+    // lane u: the word of keys equal to the prefix in step u, and how many came before it
+    auto find_same = [&](int round, int& eq, int& before) {
+        const Bits same = bits_of(round, [&](int, uint32_t key) { return key == prefix; });
+        const int n = __popcll(same), x = wave_scan(n);
+        before = eq + x - n;
+        eq += __builtin_amdgcn_readlane(x, kWave - 1);
+        return same;
+    };
+    auto find_kept = [&](int round, int& eq) {
+        if (!ties) return bits_of(round, [&](int, uint32_t key) { return key >= prefix; });
+        int before;
+        const Bits same = find_same(round, eq, before);
+        return bits_of(round, [&](int u, uint32_t key) {
+            return key > prefix || (key == prefix && below_lane(lane_bits(same, u), __builtin_amdgcn_readlane(before, u)) < left);
+        });
+    };
+    auto below_keep = [&](int round) {
+        // (a lane without a step of this wavefront has no slots)
+        const int first = s0 + (round * kWave + lane) * kWave, n = keep - first;
+        return first >= s1 || n <= 0 ? 0ull : n >= kWave ? ~0ull : (1ull << n) - 1ull;
+    };
+    int eq0 = 0;
+    if (ties) {
+        int before;
+        for (int round = 0; round < rounds; ++round) (void)find_same(round, eq0, before);
+        eq0 = __builtin_amdgcn_readfirstlane(block_scan(make_int2(lane == 0 ? eq0 : 0, 0), sums, total).x);
     }
-    __syncthreads();
-    for (int s = keep + tid; s < cap; s += kPickThreads) {
-        w_out[s] = 0.0f;
-        t_out[s] = 0;
+    int eq = eq0;
+    Bits kept = 0;
+    int2 mine = make_int2(0, 0);  // free slots below keep, moving tokens
+    for (int round = 0; round < rounds; ++round) {
+        kept = find_kept(round, eq);
+        const Bits low = below_keep(round);
+        mine.x += __popcll(low & ~kept);
+        mine.y += __popcll(kept & ~low);
+    }
+    const int2 at0 = block_scan(mine, sums, total);
+    int free0 = __builtin_amdgcn_readfirstlane(at0.x), move0 = __builtin_amdgcn_readfirstlane(at0.y);
+    eq = eq0;
+    for (int round = 0; round < rounds; ++round) {
+        if (rounds > 1) kept = find_kept(round, eq);
+        const Bits low = below_keep(round);
+        const int f = __popcll(low & ~kept), m = __popcll(kept & ~low), fs = wave_scan(f), ms = wave_scan(m);
+        const int first = s0 + round * kWave * kWave, word = first / kWave + lane, moves_before = move0 + ms - m;
+        if (word * kWave < s1) {
+            r.stays[word] = kept;
+            r.free_before[word] = free0 + fs - f;
+        }
+        const Bits move = kept & ~low;
+        const int n = min(mine_n - round * kWave, kWave);
+        for (int u = max(0, (keep - first) / kWave); u < n; ++u) {
+            const Bits v = lane_bits(move, u);
+            if (__builtin_amdgcn_inverse_ballot_w64(v)) r.from[below_lane(v, __builtin_amdgcn_readlane(moves_before, u))] = first + u * kWave + lane;
+        }
+        free0 += __builtin_amdgcn_readlane(fs, kWave - 1);
+        move0 += __builtin_amdgcn_readlane(ms, kWave - 1);
     }
 }
 
-constexpr int kMoveWaves = 4;
+constexpr int kMoveWaves = 4, kMoveThreads = kMoveWaves * kWave;
+constexpr int kClearSlots = 4 * kMoveThreads;
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 
-// Where slot s of sequence b lies: its page's record of head h, and the token in it.
-template <int BYTES>
-__device__ inline size_t page_at(const EvictArgs& a, int b, int h, int s) {
-    return ((size_t)a.table[(size_t)b * a.max_blocks + s / kPage] * a.hkv + h) * BYTES;
+__device__ inline size_t lane64(size_t v, int l) {
+    return ((size_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, l);
 }
 
-template <int HD, bool INT4>
-__global__ __launch_bounds__(kMoveWaves * kWave) void k_move(EvictArgs a) {
-    constexpr int BYTES = INT4 ? page_bytes(HD) : 2 * kPage * HD, S = HD / 32;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z;
-    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.lens_out[b] = new_lens(a)[b];
-    const int page = blockIdx.x * kMoveWaves + wave, ks = kept_slots(a.max_blocks, a.keep);
-    if (page * kPage >= ks) return;
-    // lane t < 16: where the page's slot t gets its token from
-    const int from = lane < kPage ? row_of(a, b, h).src[page * kPage + lane] : -1;
-    const unsigned moved = (unsigned)__ballot(from >= 0);
-    if (!moved) return;
-    const size_t dst = page_at<BYTES>(a, b, h, page * kPage);
-    const size_t src = from >= 0 ? page_at<BYTES>(a, b, h, from) : 0;
-    for (unsigned left = moved; left; left &= left - 1) {
-        const int t = __builtin_ctz(left), u = __builtin_amdgcn_readlane(from, t) % kPage;
-        const size_t sp = ((size_t)(uint32_t)__builtin_amdgcn_readlane((int)(src >> 32), t) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)src, t);
-        if constexpr (INT4) {
-            const uint32_t* ks32 = reinterpret_cast<const uint32_t*>(a.kpool + sp);
-            uint32_t* kd32 = reinterpret_cast<uint32_t*>(a.kpool + dst);
-            if (lane < HD / 8) kd32[t * (HD / 8) + lane] = ks32[u * (HD / 8) + lane];
-            if (lane < 2 * S) {  // scales: K's, then V's
-                uint8_t* pool = lane < S ? a.kpool : a.vpool;
-                reinterpret_cast<uint16_t*>(pool + dst + 8 * HD)[scale_at(HD, t, lane % S)] =
-                    reinterpret_cast<const uint16_t*>(pool + sp + 8 * HD)[scale_at(HD, u, lane % S)];
+// Tokens into one page of one kv head.  Lane t < 16 has the record (byte
+// offset `src`) and the slot there (`u`) of the token that slot t takes, `moved`
+// has a bit for each t that takes one.  All of a step's loads are requested
+// before its stores; a lane alone writes the words it reads.
+template <int HD>
+__device__ inline void move_f16(const EvictArgs& a, size_t dst, size_t src, int u, unsigned moved, int lane) {
+    // K: 16 bytes of a vector a lane
+    constexpr int KL = HD / 8, KT = kWave / KL < kPage ? kWave / KL : kPage, KN = kPage / KT;  // lanes of a vector, vectors and steps
+    u4_t k[KN] = {};
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+        const int t = i * KT + lane / KL;
+        const size_t p = __shfl(src, t, kWave) + 2 * HD * __shfl(u, t, kWave);
+        if (moved >> t & 1u) k[i] = reinterpret_cast<const u4_t*>(a.kpool + p)[lane % KL];
+    }
+    // V: a dimension's 16 tokens a lane, as one row
+    constexpr int VN = HD / kWave;
+    uint16_t v[kPage][VN] = {};
+    u4_t row[VN][2];
+#pragma unroll
+    for (int i = 0; i < VN; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) row[i][j] = reinterpret_cast<const u4_t*>(a.vpool + dst)[2 * (i * kWave + lane) + j];
+#pragma unroll
+    for (int t = 0; t < kPage; ++t)
+        if (moved >> t & 1u) {
+            const uint16_t* from = reinterpret_cast<const uint16_t*>(a.vpool + lane64(src, t)) + __builtin_amdgcn_readlane(u, t);
+#pragma unroll
+            for (int i = 0; i < VN; ++i) v[t][i] = from[(i * kWave + lane) * kPage];
+        }
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+        const int t = i * KT + lane / KL;
+        if (moved >> t & 1u) reinterpret_cast<u4_t*>(a.kpool + dst + 2 * HD * t)[lane % KL] = k[i];
+    }
+#pragma unroll
+    for (int t = 0; t < kPage; ++t)
+        if (moved >> t & 1u)
+#pragma unroll
+            for (int i = 0; i < VN; ++i) {
+                uint32_t w = row[i][t / 8][t / 2 % 4];
+                w = t % 2 ? (w & 0xFFFFu) | (uint32_t)v[t][i] << 16 : (w & 0xFFFF0000u) | v[t][i];
+                row[i][t / 8][t / 2 % 4] = w;
             }
-            // V: lane n < 16 of quad t / 4 takes the two nibbles of its S dwords
-            if (lane >> 4 == t >> 2) {
-                const uint32_t* vs32 = reinterpret_cast<const uint32_t*>(a.vpool + sp);
-                uint32_t* vd32 = reinterpret_cast<uint32_t*>(a.vpool + dst);
 #pragma unroll
-                for (int i = 0; i < S; ++i) {
-                    const uint32_t w = vs32[(16 * (u >> 2) + (lane & 15)) * S + i];
-                    uint32_t d = vd32[lane * S + i];
+    for (int i = 0; i < VN; ++i)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int ns = 4 * v_nib(u, 16 * e), nd = 4 * v_nib(t, 16 * e);
-                        d = (d & ~(15u << nd)) | ((w >> ns & 15u) << nd);
-                    }
-                    vd32[lane * S + i] = d;
+        for (int j = 0; j < 2; ++j) reinterpret_cast<u4_t*>(a.vpool + dst)[2 * (i * kWave + lane) + j] = row[i][j];
+}
+
+template <int HD>
+__device__ inline void move_int4(const EvictArgs& a, size_t dst, size_t src, int u, unsigned moved, int lane) {
+    constexpr int S = HD / 32;
+    // K: 16 bytes of a token's codes a lane
+    constexpr int KL = HD / 32, KT = kWave / KL < kPage ? kWave / KL : kPage, KN = kPage / KT;
+    u4_t k[KN] = {};
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+        const int t = i * KT + lane / KL;
+        const size_t p = __shfl(src, t & 15, kWave) + HD / 2 * __shfl(u, t & 15, kWave);
+        if (t < kPage && (moved >> t & 1u)) k[i] = reinterpret_cast<const u4_t*>(a.kpool + p)[lane % KL];
+    }
+    // scales: a token's S of K, then of V
+    constexpr int SN = 2 * S * kPage / kWave;
+    uint16_t sc[SN] = {};
+#pragma unroll
+    for (int i = 0; i < SN; ++i) {
+        const int x = i * kWave + lane, t = x / (2 * S), g = x % (2 * S);
+        const size_t p = __shfl(src, t, kWave);
+        const int from = __shfl(u, t, kWave);
+        if (moved >> t & 1u) sc[i] = reinterpret_cast<const uint16_t*>((g < S ? a.kpool : a.vpool) + p + 8 * HD)[scale_at(HD, from, g % S)];
+    }
+    // V: lane (g, n) has the S dwords of quad g, and of its four tokens the
+    // dwords that hold them elsewhere
+    const int q = lane >> 4, n = lane & 15;
+    uint32_t* own = reinterpret_cast<uint32_t*>(a.vpool + dst) + lane * S;
+    const bool mine = moved >> (4 * q) & 15u;
+    uint32_t d[S] = {}, w[4][S] = {};
+    int from[4];
+    if (mine)
+#pragma unroll
+        for (int i = 0; i < S; ++i) d[i] = own[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const size_t p = __shfl(src, 4 * q + j, kWave);
+        from[j] = __shfl(u, 4 * q + j, kWave);
+        if (moved >> (4 * q + j) & 1u)
+#pragma unroll
+            for (int i = 0; i < S; ++i) w[j][i] = reinterpret_cast<const uint32_t*>(a.vpool + p)[(16 * (from[j] >> 2) + n) * S + i];
+    }
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+        const int t = i * KT + lane / KL;
+        if (t < kPage && (moved >> t & 1u)) reinterpret_cast<u4_t*>(a.kpool + dst + HD / 2 * t)[lane % KL] = k[i];
+    }
+#pragma unroll
+    for (int i = 0; i < SN; ++i) {
+        const int x = i * kWave + lane, t = x / (2 * S), g = x % (2 * S);
+        if (moved >> t & 1u) reinterpret_cast<uint16_t*>((g < S ? a.kpool : a.vpool) + dst + 8 * HD)[scale_at(HD, t, g % S)] = sc[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (moved >> (4 * q + j) & 1u)
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int ns = 4 * v_nib(from[j], 16 * e), nd = 4 * v_nib(j, 16 * e);
+                    d[i] = (d[i] & ~(15u << nd)) | ((w[j][i] >> ns & 15u) << nd);
                 }
-            }
-        } else {
-            const uint4* k4 = reinterpret_cast<const uint4*>(a.kpool + sp);
-            uint4* kd4 = reinterpret_cast<uint4*>(a.kpool + dst);
-            if (lane < HD / 8) kd4[t * (HD / 8) + lane] = k4[u * (HD / 8) + lane];
-            const uint16_t* vs = reinterpret_cast<const uint16_t*>(a.vpool + sp);
-            uint16_t* vd = reinterpret_cast<uint16_t*>(a.vpool + dst);
-            for (int d = lane; d < HD; d += kWave) vd[d * kPage + t] = vs[d * kPage + u];
+    if (mine)
+#pragma unroll
+        for (int i = 0; i < S; ++i) own[i] = d[i];
+}
+
+// The first blocks of a (kv head, sequence) take kMoveWaves pages of kept slots
+// each, the others clear kClearSlots slots' weights and tags beyond them.  The
+// weights' outputs may be their inputs: a slot that a token leaves is cleared
+// by the lane that has read it, every other by its own.
+template <int HD, bool INT4>
+__global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
+    constexpr int BYTES = INT4 ? page_bytes(HD) : 2 * kPage * HD;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z;
+    const Seq seq = *seq_of(a, b);
+    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.lens_out[b] = seq.len;
+    if (seq.len < 0) return;
+    const int cap = a.max_blocks * kPage, ks = kept_slots(a.max_blocks, a.keep), blocks = (ks / kPage + kMoveWaves - 1) / kMoveWaves;
+    const size_t at = ((size_t)b * a.hkv + h) * cap;
+    const Row r = row_of(a, b, h);
+    const int tokens = seq.cut ? a.seen[b] - seq.ahead + 1 : seq.len;  // cached before
+    if ((int)blockIdx.x >= blocks) {
+        const int first = ks + ((int)blockIdx.x - blocks) * kClearSlots, end = min(cap, first + kClearSlots);
+        for (int s = first + (int)threadIdx.x; s < end; s += kMoveThreads) {
+            if (s < tokens && (r.stays[s / kWave] >> (s % kWave) & 1ull)) continue;
+            a.weights_out[at + s] = 0.0f;
+            a.tags_out[at + s] = 0;
         }
+        return;
+    }
+    const int page = blockIdx.x * kMoveWaves + wave;
+    if (page * kPage >= ks) return;
+    // lane t < 16: slot t of the page
+    const int s = page * kPage + (lane & 15), bit = s % kWave;
+    const bool used = s < seq.len && lane < kPage;
+    unsigned long long stays = ~0ull;
+    int free_before = 0;
+    if (seq.cut) {
+        stays = r.stays[page * kPage / kWave];
+        free_before = r.free_before[page * kPage / kWave];
+    }
+    const bool takes = used && !(stays >> bit & 1ull);
+    int from = 0, tag = 0;
+    float w = 0.0f;
+    if (used) {
+        from = takes ? r.from[free_before + __popcll(~stays & ((1ull << bit) - 1ull))] : s;
+        const int t = a.tags_in[at + from];
+        tag = t > 0 ? t : seq.ahead + from;
+        w = a.weights_in[at + from];
+    }
+    const unsigned moved = (unsigned)__ballot(takes);
+    if (moved) {
+        const int32_t* table = a.table + (size_t)b * a.max_blocks;
+        const size_t src = takes ? ((size_t)table[from / kPage] * a.hkv + h) * BYTES : 0;
+        const size_t dst = ((size_t)table[page] * a.hkv + h) * BYTES;
+        if constexpr (INT4)
+            move_int4<HD>(a, dst, src, from % kPage, moved, lane);
+        else
+            move_f16<HD>(a, dst, src, from % kPage, moved, lane);
+    }
+    if (lane < kPage && (used || s >= tokens || !(stays >> bit & 1ull))) {
+        a.weights_out[at + s] = w;
+        a.tags_out[at + s] = tag;
+    }
+    if (takes) {
+        a.weights_out[at + from] = 0.0f;
+        a.tags_out[at + from] = 0;
     }
 }
 
 template <int HD, bool INT4>
 void move_case(const EvictArgs& a, hipStream_t st) {
-    const int pages = kept_slots(a.max_blocks, a.keep) / kPage;
-    hipLaunchKernelGGL((k_move<HD, INT4>), dim3((unsigned)((pages + kMoveWaves - 1) / kMoveWaves), (unsigned)a.hkv, (unsigned)a.batch),
-                       dim3(kMoveWaves * kWave), 0, st, a);
+    const int ks = kept_slots(a.max_blocks, a.keep), rest = a.max_blocks * kPage - ks;
+    const unsigned blocks = (unsigned)((ks / kPage + kMoveWaves - 1) / kMoveWaves + (rest + kClearSlots - 1) / kClearSlots);
+    hipLaunchKernelGGL((k_move<HD, INT4>), dim3(blocks, (unsigned)a.hkv, (unsigned)a.batch), dim3(kMoveThreads), 0, st, a);
 }
 
 }  // namespace
 
 size_t evict_ws_words(int batch, int hkv, int max_blocks, int keep) {
-    return (size_t)batch * hkv * ((size_t)max_blocks * kPage + 2 * (size_t)kept_slots(max_blocks, keep)) + batch;
+    return (size_t)batch * kSeqWords + (size_t)batch * hkv * row_words(max_blocks, keep);
 }
 
 hipError_t evict_launch(const EvictArgs& a, bool int4, hipStream_t st) {
     if (a.hd != 64 && a.hd != 128 && a.hd != 256) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_pick, dim3((unsigned)a.hkv, (unsigned)a.batch), dim3(kPickThreads), 0, st, a);
+    const dim3 rows((unsigned)a.hkv, (unsigned)a.batch), threads(kPickThreads);
+    const int cap = a.max_blocks * kPage;
+    if (cap <= 8192)
+        hipLaunchKernelGGL(k_pick<8192>, rows, threads, 0, st, a);
+    else if (cap <= kLdsSlots)
+        hipLaunchKernelGGL(k_pick<kLdsSlots>, rows, threads, 0, st, a);
+    else
+        hipLaunchKernelGGL(k_pick<0>, rows, threads, 0, st, a);
     if (a.hd == 64)
         int4 ? move_case<64, true>(a, st) : move_case<64, false>(a, st);
     else if (a.hd == 128)
