@@ -33,7 +33,6 @@ namespace kvc {
 
 namespace {
 
-using at::as_h8;
 using at::f4_t;
 using at::h8_t;
 
@@ -41,86 +40,104 @@ constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kMaxSplits = 64;
 constexpr int kRowRor8 = 0x128;
-// Probabilities are exp2(s - max + kUp): up to 2^15 instead of 1, so that the
-// small ones stay normal fp16 numbers (below 2^-14 fp16 loses bits).  L is the
-// sum of the same values, and O / L does not see the factor.
 constexpr float kUp = 15.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------------- pages --
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+
 // A lane's share of a pair of pages.
 template <int HD>
 struct PairI4 {
     uint32_t k[2][HD / 32], v[2][HD / 32];  // codes: K of token l%16, V of tokens 4 g .. +3
-    uint2 ks[2][HD / 32], vs[2][HD / 32];   // scales of tokens 4 g .. +3 per group
+    h4_t ks[2][HD / 32], vs[2][HD / 32];    // scales of tokens 4 g .. +3 per group
 };
 
 // N dwords that start at a multiple of 4 N bytes (of 16 where N is above 4).
 template <int N>
 __device__ inline void load_words(uint32_t (&r)[N], const uint8_t* p) {
     if constexpr (N == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        const u2_t w = *reinterpret_cast<const u2_t*>(p);
         r[0] = w.x, r[1] = w.y;
     } else {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const uint4 w = reinterpret_cast<const uint4*>(p)[i / 4];
+            const u4_t w = reinterpret_cast<const u4_t*>(p)[i / 4];
             r[i] = w.x, r[i + 1] = w.y, r[i + 2] = w.z, r[i + 3] = w.w;
         }
     }
 }
 template <int N>
-__device__ inline void load_pairs(uint2 (&r)[N], const uint8_t* p) {
+__device__ inline void load_scales(h4_t (&r)[N], const uint8_t* p) {
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const uint4 w = reinterpret_cast<const uint4*>(p)[i / 2];
-        r[i] = make_uint2(w.x, w.y), r[i + 1] = make_uint2(w.z, w.w);
+        const h8_t w = reinterpret_cast<const h8_t*>(p)[i / 2];
+        r[i] = __builtin_shufflevector(w, w, 0, 1, 2, 3), r[i + 1] = __builtin_shufflevector(w, w, 4, 5, 6, 7);
     }
 }
 
 template <int HD>
-__device__ inline void load_pair(PairI4<HD>& r, const AttnArgs& a, int blka, int blkb, int kvh, int lane) {
+__device__ inline void load_k(PairI4<HD>& r, const AttnArgs& a, const int (&blk)[2], int kvh, int lane) {
     constexpr int S = HD / 32;
-    const int g = lane >> 4, t = lane & 15;
+    const uint32_t g = lane >> 4, t = lane & 15;
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
-        const size_t base = ((size_t)(pg ? blkb : blka) * a.hkv + kvh) * page_bytes(HD);
-        load_words<S>(r.k[pg], a.kpool + base + (t * 4 + g) * (4 * S));
-        load_pairs<S>(r.ks[pg], a.kpool + base + 8 * HD + g * (8 * S));
-        load_words<S>(r.v[pg], a.vpool + base + lane * (4 * S));
-        load_pairs<S>(r.vs[pg], a.vpool + base + 8 * HD + g * (8 * S));
+        const uint8_t* p = a.kpool + ((size_t)(uint32_t)blk[pg] * (uint32_t)a.hkv + (uint32_t)kvh) * page_bytes(HD);
+        load_words<S>(r.k[pg], p + (t * 4 + g) * (4 * S));
+        load_scales<S>(r.ks[pg], p + 8 * HD + g * (8 * S));
+    }
+}
+template <int HD>
+__device__ inline void load_v(PairI4<HD>& r, const AttnArgs& a, const int (&blk)[2], int kvh, int lane) {
+    constexpr int S = HD / 32;
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg) {
+        const uint8_t* p = a.vpool + ((size_t)(uint32_t)blk[pg] * (uint32_t)a.hkv + (uint32_t)kvh) * page_bytes(HD);
+        load_words<S>(r.v[pg], p + (uint32_t)lane * (4 * S));
+        load_scales<S>(r.vs[pg], p + 8 * HD + ((uint32_t)lane >> 4) * (8 * S));
     }
 }
 
 template <int HD>
 struct PairF16 {
-    uint4 k[2][HD / 32];
-    uint2 v[HD / 16][2];
+    h8_t k[2][HD / 32];
+    u2_t v[HD / 16][2];
 };
 
 template <int HD>
-__device__ inline void load_pair(PairF16<HD>& r, const AttnArgs& a, int blka, int blkb, int kvh, int lane) {
-    const int g = lane >> 4, t = lane & 15;
+__device__ inline void load_k(PairF16<HD>& r, const AttnArgs& a, const int (&blk)[2], int kvh, int lane) {
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
-        const size_t base = ((size_t)(pg ? blkb : blka) * a.hkv + kvh) * (2 * kPage * HD);
+        const uint8_t* p = a.kpool + ((size_t)(uint32_t)blk[pg] * (uint32_t)a.hkv + (uint32_t)kvh) * (2 * kPage * HD);
 #pragma unroll
-        for (int s = 0; s < HD / 32; ++s)
-            r.k[pg][s] = *reinterpret_cast<const uint4*>(a.kpool + base + 2 * (t * HD + 32 * s + 8 * g));
+        for (int s = 0; s < HD / 32; ++s) r.k[pg][s] = *reinterpret_cast<const h8_t*>(p + 2u * ((lane & 15u) * HD + 8u * ((uint32_t)lane >> 4)) + 64 * s);
+    }
+}
+template <int HD>
+__device__ inline void load_v(PairF16<HD>& r, const AttnArgs& a, const int (&blk)[2], int kvh, int lane) {
 #pragma unroll
-        for (int nt = 0; nt < HD / 16; ++nt)
-            r.v[nt][pg] = *reinterpret_cast<const uint2*>(a.vpool + base + 2 * ((16 * nt + t) * kPage + 4 * g));
+    for (int pg = 0; pg < 2; ++pg) {
+        const uint8_t* p = a.vpool + ((size_t)(uint32_t)blk[pg] * (uint32_t)a.hkv + (uint32_t)kvh) * (2 * kPage * HD);
+#pragma unroll
+        for (int nt = 0; nt < HD / 16; ++nt) r.v[nt][pg] = *reinterpret_cast<const u2_t*>(p + 2u * ((lane & 15u) * kPage + 4u * ((uint32_t)lane >> 4)) + 32 * kPage * nt);
     }
 }
 
 // Codes of half a dword (nibbles 0 and 4, 1 and 5) as fp16 values code - 8:
 // 0x6400 is 1024, whose last bits a nibble sets; both steps are exact.
+__device__ inline uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t v;  // (the compiler takes two instructions for it, as two of the operands are constants)
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(v) : "v"(w), "s"(mask), "v"(bits));
+    return v;
+}
 __device__ inline half2_t low_codes(uint32_t w) {
-    const half2_t v = __builtin_bit_cast(half2_t, (w & 0x000F000Fu) | 0x64006400u);
+    const half2_t v = __builtin_bit_cast(half2_t, and_or(w, 0x000F000Fu, 0x64006400u));
     return v + half2_t{(_Float16)-1032.0f, (_Float16)-1032.0f};
 }
 __device__ inline half2_t high_codes(uint32_t w) {  // 1024 + 16 code
-    const half2_t v = __builtin_bit_cast(half2_t, (w & 0x00F000F0u) | 0x64006400u);
+    const half2_t v = __builtin_bit_cast(half2_t, and_or(w, 0x00F000F0u, 0x64006400u));
     return __builtin_elementwise_fma(v, half2_t{(_Float16)0.0625f, (_Float16)0.0625f}, half2_t{(_Float16)-72.0f, (_Float16)-72.0f});
 }
 struct H2x4 {
@@ -130,89 +147,111 @@ __device__ inline h8_t codes8(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(h8_t, H2x4{low_codes(a), high_codes(a), low_codes(b), high_codes(b)});
 }
 
-__device__ inline float half_of(uint2 w, int i) { return h2f_bits((uint16_t)((i < 2 ? w.x : w.y) >> (16 * (i & 1)))); }
-
 // ------------------------------------------------------------ scores of a pair --
 template <int HD>
-__device__ inline void scores(const PairI4<HD>& r, const h8_t (&q)[HD / 32], f4_t (&s)[2]) {
+__device__ inline void scores(const PairI4<HD>& r, const h8_t* q, f4_t (&s)[2]) {
+    s[0] = s[1] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int pg = 0; pg < 2; ++pg) {
-        f4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < HD / 32; ++i) {
+        const h8_t qi = q[i * kWave];
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
+        for (int pg = 0; pg < 2; ++pg) {
             const h8_t k = codes8(r.k[pg][i], r.k[pg][i] >> 8);
-            const f4_t d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[i], f4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            const f4_t d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qi, f4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = fmaf(d[j], half_of(r.ks[pg][i], j), acc[j]);
+            for (int j = 0; j < 4; ++j) s[pg][j] = __builtin_fmaf(d[j], (float)r.ks[pg][i][j], s[pg][j]);
         }
-        s[pg] = acc;
+        if (i % 2) __builtin_amdgcn_sched_barrier(0);
     }
 }
 
 template <int HD>
-__device__ inline void scores(const PairF16<HD>& r, const h8_t (&q)[HD / 32], f4_t (&s)[2]) {
+__device__ inline void scores(const PairF16<HD>& r, const h8_t* q, f4_t (&s)[2]) {
+    s[0] = s[1] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int pg = 0; pg < 2; ++pg) {
-        f4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < HD / 32; ++i) {
+        const h8_t qi = q[i * kWave];
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(r.k[pg][i]), q[i], acc, 0, 0, 0);
-        s[pg] = acc;
+        for (int pg = 0; pg < 2; ++pg) s[pg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.k[pg][i], qi, s[pg], 0, 0, 0);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-// ------------------------------------------------------------ values of a pair --
-// o += P V.  p: probabilities of tokens 4 g + j of page a (j < 4) and page b.
-// The product takes p times the token's scale, rounded to fp16: at most
-// 2^-11 of a term, which stays linear in the output (an fp16 number itself).
-// p is up to 2^15, so a scale of 2 or more (a value of 16 and up among a
-// group) could pass the largest fp16 number: such a pair goes without the factor
-// 2^15 and its sums get it afterwards.
+// Tokens past a page's valid ones may hold anything, and their probability, 0,
+// must not meet a NaN: the int4 scales and the fp16 values become zeros.
 template <int HD>
-__device__ inline void values(const PairI4<HD>& r, const float (&p)[8], int na, int nb, f4_t (&o)[HD / 16], int lane) {
-    constexpr int S = HD / 32;
-    const int g = lane >> 4;
-    uint2 vs[2][S];
-    uint32_t seen = 0u;
-    // scales of tokens past the page's valid ones may be anything
-    const uint2 m[2] = {at::vmask_of(na, g), at::vmask_of(nb, g)};
+__device__ inline void clear_past(PairI4<HD>& r, int na, int nb, int lane) {
+    const uint2 m[2] = {at::vmask_of(na, lane >> 4), at::vmask_of(nb, lane >> 4)};
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            vs[pg][i] = make_uint2(r.vs[pg][i].x & m[pg].x, r.vs[pg][i].y & m[pg].y);
-            seen |= vs[pg][i].x | vs[pg][i].y;
-        }
-    const bool large = __any((seen & 0x40004000u) != 0u);  // an exponent of 2^1 and up
-    const float down = large ? 1.0f / 32768.0f : 1.0f;
+        for (int i = 0; i < HD / 32; ++i)
+            r.vs[pg][i] = __builtin_bit_cast(h4_t, __builtin_bit_cast(u2_t, r.vs[pg][i]) & u2_t{m[pg].x, m[pg].y});
+}
+template <int HD>
+__device__ inline void clear_past(PairF16<HD>& r, int na, int nb, int lane) {
+    const uint2 m[2] = {at::vmask_of(na, lane >> 4), at::vmask_of(nb, lane >> 4)};
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
+    for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+        for (int nt = 0; nt < HD / 16; ++nt) r.v[nt][pg] &= u2_t{m[pg].x, m[pg].y};
+}
+
+// One wavefront's state over its pairs of pages: a column's running maximum (of
+// scores times log2 e), this lane's part of its sum, and O.  Probabilities are
+// exp2(s - max + up), up to 2^15 instead of 1, so that small ones stay normal
+// fp16 numbers (below 2^-14 fp16 loses bits); L and O have the same factor.
+template <int HD>
+struct Fold {
+    float m = -__builtin_inff(), l = 0.0f, up = kUp;
+    f4_t o[HD / 16];
+};
+
+// ------------------------------------------------------------ values of a pair --
+// The powers of two that the probabilities of a pair may have.  P V takes p
+// times the token's scale, rounded to fp16: at most 2^-11 of a term, which
+// stays linear in the output (an fp16 number itself).  With p up to 2^15 a
+// scale of 2 or more (a value of 16 and up among a group) could pass the
+// largest fp16 number: from such a pair on the wavefront's factor is as many
+// powers of two smaller.
+template <int HD>
+__device__ inline float most_up(const PairI4<HD>& r, float up) {
+    typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
+    typedef uint16_t us4_t __attribute__((ext_vector_type(4)));
+    us2_t most = {0, 0};
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+            const us4_t w = __builtin_bit_cast(us4_t, r.vs[pg][i]);
+            most = __builtin_elementwise_max(most, __builtin_elementwise_max(__builtin_shufflevector(w, w, 0, 1), __builtin_shufflevector(w, w, 2, 3)));
+        }
+    const int e = max((int)most.x, (int)most.y) >> 10;  // biased exponent: 15 is 2^0
+    return __any(e > 30 - (int)up) ? 30.0f - wave_max((float)e) : up;
+}
+template <int HD>
+__device__ inline float most_up(const PairF16<HD>&, float up) {
+    return up;
+}
+
+// o += P V.  p: probabilities of tokens 4 g + j of page a (j < 4) and page b.
+template <int HD>
+__device__ inline void values(const PairI4<HD>& r, const float (&p)[8], f4_t (&o)[HD / 16], int) {
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
         h8_t ps;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float sc = half_of(vs[j / 4][i], j % 4);
-            ps[j] = (_Float16)(large ? p[j] * down * sc : p[j] * sc);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const uint32_t wa = e ? r.v[0][i] >> 8 : r.v[0][i], wb = e ? r.v[1][i] >> 8 : r.v[1][i];
-            const h8_t v = codes8(wa, wb);
-            f4_t& acc = o[2 * i + e];
-            if (large) {
-                const f4_t d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps, v, f4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j] = fmaf(d[j], 32768.0f, acc[j]);
-            } else {
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps, v, acc, 0, 0, 0);
-            }
-        }
+        for (int j = 0; j < 8; ++j) ps[j] = (_Float16)__builtin_fmaf(p[j], (float)r.vs[j / 4][i][j % 4], 0.0f);
+        o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps, codes8(r.v[0][i], r.v[1][i]), o[2 * i], 0, 0, 0);
+        o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps, codes8(r.v[0][i] >> 8, r.v[1][i] >> 8), o[2 * i + 1], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
 // fp16 pages: rows 0-7 of the product take the fp16 high parts of the heads'
 // probabilities and rows 8-15 (the lanes of columns 8-15) the low parts.
 template <int HD>
-__device__ inline void values(const PairF16<HD>& r, const float (&p)[8], int na, int nb, f4_t (&o)[HD / 16], int lane) {
-    const int g = lane >> 4;
+__device__ inline void values(const PairF16<HD>& r, const float (&p)[8], f4_t (&o)[HD / 16], int lane) {
     const bool low = lane & 8;
     h8_t ps;
 #pragma unroll
@@ -220,19 +259,119 @@ __device__ inline void values(const PairF16<HD>& r, const float (&p)[8], int na,
         const _Float16 hi = (_Float16)p[j];
         ps[j] = low ? (_Float16)(p[j] - (float)hi) : hi;
     }
-    // V words of tokens past the valid ones may be anything
-    const uint2 ma = at::vmask_of(na, g), mb = at::vmask_of(nb, g);
 #pragma unroll
     for (int nt = 0; nt < HD / 16; ++nt) {
-        const h8_t v = as_h8(make_uint4(r.v[nt][0].x & ma.x, r.v[nt][0].y & ma.y, r.v[nt][1].x & mb.x, r.v[nt][1].y & mb.y));
+        const h8_t v = __builtin_bit_cast(h8_t, __builtin_shufflevector(r.v[nt][0], r.v[nt][1], 0, 1, 2, 3));
         o[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps, v, o[nt], 0, 0, 0);
     }
 }
 
 // ------------------------------------------------------------------- k_attn --
+// q as operands in LDS, by the whole block: [step][lane] 8 fp16 values.  Column
+// t < 8 is the high part of head h0 + t (zero past H), column 8 + t its low
+// part.  A power of two per head brings its largest value to 512 and up, so
+// that low parts are normal fp16 numbers and no high part overflows; scale[t]
+// takes it back.
+template <int HD>
+__device__ inline void stage_q(const float* q, int H, _Float16* ops, float* scale) {
+    constexpr int T = HD / 4;  // threads of a head, four dimensions each
+    static_assert(T * kHeadsPerBlock <= kThreads && T <= kWave && kWave % T == 0, "a head lies in one wavefront");
+    const int h = threadIdx.x / T, d = 4 * (threadIdx.x % T);
+    if (h >= kHeadsPerBlock) return;
+    const f4_t x = h < H ? *reinterpret_cast<const f4_t*>(q + (size_t)h * HD + d) : f4_t{0.f, 0.f, 0.f, 0.f};
+    float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+    for (int o = 1; o < T; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
+    const int up = e == 0 || e == 255 ? 0 : min(136 - e, 126);
+    h4_t hi, lo;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float y = ldexpf(x[j], up);
+        hi[j] = (_Float16)y;
+        lo[j] = (_Float16)(y - (float)hi[j]);
+    }
+    const int at = ((d / 32) * kWave + 16 * (d % 32 / 8)) * 8 + d % 8;
+    *reinterpret_cast<h4_t*>(ops + at + 8 * h) = hi;
+    *reinterpret_cast<h4_t*>(ops + at + 8 * (h + 8)) = lo;
+    if (d == 0) scale[h] = ldexpf(kLog2e / sqrtf((float)HD), -up);
+}
+
+// Maximum over the four lanes of a column (lanes l, l ^ 16, l ^ 32, l ^ 48).
+__device__ inline float column_max(float v) {
+    typedef uint32_t __attribute__((ext_vector_type(2))) pair_t;
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const pair_t a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t x0 = a[0], x1 = a[1];
+    const float m = fmaxf(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1));
+    const uint32_t w = __builtin_bit_cast(uint32_t, m);
+    const pair_t b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    const uint32_t y0 = b[0], y1 = b[1];
+    return fmaxf(__builtin_bit_cast(float, y0), __builtin_bit_cast(float, y1));
+}
+
+// A pair of pages into the state.  The next pair's K is requested once this
+// one's has become scores, its V once this one's is added: half a pair is in
+// flight all the time, in registers that are free anyway.
+template <int HD, bool ACC, class Pair, class Next>
+__device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, float scale, int na, int nb, float* raw, int lane, Next next_k) {
+    const int g = lane >> 4;
+    f4_t s[2];
+    scores<HD>(r, q, s);
+    // (here, not after the next request, whose registers these were)
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]));
+    next_k();
+    float p[8], top = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = s[j / 4][j % 4] + dpp<kRowRor8>(s[j / 4][j % 4]);
+    if (nb < kPage) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = 4 * g + j % 4 < (j < 4 ? na : nb) ? p[j] : -__builtin_inff();
+        clear_past<HD>(r, na, nb, lane);
+    }
+    if constexpr (ACC) {
+        if (raw) {
+            reinterpret_cast<f4_t*>(raw)[0] = f4_t{p[0], p[1], p[2], p[3]} * scale;
+            if (nb > 0) reinterpret_cast<f4_t*>(raw)[4] = f4_t{p[4], p[5], p[6], p[7]} * scale;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, p[j]);
+    top = column_max(top) * scale;
+    const float mn = fmaxf(f.m, top);
+    const bool none = mn == -__builtin_inff();  // no token, or NaN scores alone
+    const float up = most_up<HD>(r, f.up);
+    const float corr = none ? 1.0f : __builtin_amdgcn_exp2f(f.m - mn + (up - f.up)), from = none ? 0.0f : mn - up;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], scale, -from));
+        sum += p[j];
+    }
+    f.l = f.l * corr + sum;
+    // rows of O are heads: their factors lie in the lanes of that column (there
+    // is no O yet where the maximum was not one)
+    if (__any(corr != 1.0f && f.m != -__builtin_inff())) {
+        float c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = __shfl(corr, 4 * g + j, 64);
+#pragma unroll
+        for (int nt = 0; nt < HD / 16; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f.o[nt][j] *= c[j];
+    }
+    f.m = mn;
+    f.up = up;
+    values<HD>(r, p, f.o, lane);
+}
+
 template <int HD, bool INT4, bool ACC>
-__global__ __launch_bounds__(kThreads) void k_attn(AttnArgs a) {
-    __shared__ __align__(16) float lds[kWaves * kHeadsPerBlock * (HD + 2)];
+__global__ __launch_bounds__(kThreads, 2) void k_attn(AttnArgs a) {
+    using Pair = typename std::conditional<INT4, PairI4<HD>, PairF16<HD>>::type;
+    constexpr int kRec = kHeadsPerBlock * (HD + 2);
+    __shared__ __align__(16) float lds[kWaves * kRec];
+    __shared__ h8_t qops[HD / 32 * kWave];
+    __shared__ float qscale[kHeadsPerBlock];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, t = lane & 15;
     const int split = blockIdx.x, kvh = blockIdx.y / a.plan.groups, grp = blockIdx.y % a.plan.groups, b = blockIdx.z;
@@ -241,113 +380,61 @@ __global__ __launch_bounds__(kThreads) void k_attn(AttnArgs a) {
     int ctx = a.lens[b];
     bool bad = ctx < 0 || ctx > cap;
     ctx = bad ? 0 : ctx;
-    // q: column t % 8 is head h0 + t % 8 (zero past H), the low part from
-    // column 8 on.  A power of two per head brings its largest value to 512 and
-    // up, so that low parts are normal fp16 numbers and no high part overflows.
-    h8_t q[HD / 32];
-    float scale = kLog2e / sqrtf((float)HD);
-    {
-        const bool on = (t & 7) < H;
-        const float* src = a.q + ((size_t)b * a.hq + h0 + (on ? t & 7 : 0)) * HD + 8 * g;
-        float x[HD / 32][8], top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-            const float4 lo = reinterpret_cast<const float4*>(src + 32 * i)[0], hi = reinterpret_cast<const float4*>(src + 32 * i)[1];
-            const float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[i][j] = y[j];
-                top = fmaxf(top, fabsf(y[j]));
-            }
-        }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
-        const int up = e == 0 || e == 255 ? 0 : min(136 - e, 126);
-        scale = ldexpf(scale, -up);
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = ldexpf(x[i][j], up);
-                const _Float16 hi = (_Float16)y;
-                const _Float16 v = t < 8 ? hi : (_Float16)(y - (float)hi);
-                q[i][j] = on ? v : (_Float16)0.0f;
-            }
-    }
     const int npages = (ctx + kPage - 1) / kPage, npairs = (npages + 1) / 2;
     const int stride = a.plan.splits * kWaves, first = split + a.plan.splits * wave;
     const int mine = first < npairs ? (npairs - first + stride - 1) / stride : 0;
-    float m = -__builtin_inff(), l = 0.0f;
-    f4_t o[HD / 16];
-#pragma unroll
-    for (int nt = 0; nt < HD / 16; ++nt) o[nt] = f4_t{0.f, 0.f, 0.f, 0.f};
-    for (int base = 0; base < mine; base += kWave / 2) {
-        // the table entries of the next 32 pairs, two lanes each
-        const int my_page = 2 * (first + stride * (base + lane / 2)) + (lane & 1);
-        int entry = my_page < npages ? a.table[(size_t)b * a.max_blocks + my_page] : 0;
-        const bool out = entry < 0 || entry >= a.num_blocks;
-        bad = bad || __any(out);
-        entry = out ? 0 : entry;
-        const int n = min(mine - base, kWave / 2);
-        for (int i = 0; i < n; ++i) {
-            const int page = 2 * (first + stride * (base + i));
-            const int na = min(ctx - page * kPage, kPage), nb = min(max(ctx - (page + 1) * kPage, 0), kPage);
-            const int blka = __builtin_amdgcn_readlane(entry, 2 * i), blkb = nb > 0 ? __builtin_amdgcn_readlane(entry, 2 * i + 1) : blka;
-            typename std::conditional<INT4, PairI4<HD>, PairF16<HD>>::type r;
-            load_pair<HD>(r, a, blka, blkb, kvh, lane);
-            f4_t s[2];
-            scores<HD>(r, q, s);
-            float p[8];
-            float top = -__builtin_inff();
-#pragma unroll
-            for (int pg = 0; pg < 2; ++pg)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float x = (s[pg][j] + dpp<kRowRor8>(s[pg][j])) * scale;
-                    p[4 * pg + j] = 4 * g + j < (pg ? nb : na) ? x : -__builtin_inff();
-                    top = fmaxf(top, p[4 * pg + j]);
-                }
-            if constexpr (ACC) {
-                if (t < H) {
-                    float4* dst = reinterpret_cast<float4*>(a.raw + ((size_t)b * a.hq + h0 + t) * cap + page * kPage + 4 * g);
-                    dst[0] = make_float4(p[0], p[1], p[2], p[3]);
-                    if (nb > 0) dst[4] = make_float4(p[4], p[5], p[6], p[7]);
-                }
-            }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m, top);
-            const bool none = mn == -__builtin_inff();
-            const float corr = none ? 1.0f : __builtin_amdgcn_exp2f(m - mn), at0 = mn - kUp;
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                p[j] = none ? (p[j] == p[j] ? 0.0f : p[j]) : __builtin_amdgcn_exp2f(p[j] - at0);
-                sum += p[j];
-            }
-            l = l * corr + sum;
-            m = mn;
-            // rows of O are heads: their factors lie in the lanes of that column
-            if (__any(corr != 1.0f)) {
-                float c[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) c[j] = __shfl(corr, 4 * g + j, 64);
-#pragma unroll
-                for (int nt = 0; nt < HD / 16; ++nt)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[nt][j] *= c[j];
-            }
-            values<HD>(r, p, na, nb, o, lane);
+    const int32_t* table = a.table + (size_t)b * a.max_blocks;
+    int entry = 0, blk[2];
+    Pair r;
+    // the pages of pair i of this wavefront, in order
+    auto turn_to = [&](int i) {
+        if (i % (kWave / 2) == 0) {  // the table entries of the next 32 pairs, two lanes each
+            const int page = 2 * (first + stride * (i + lane / 2)) + (lane & 1);
+            entry = page < npages ? table[page] : 0;
+            const bool out = entry < 0 || entry >= a.num_blocks;
+            bad = bad || __any(out);
+            entry = out ? 0 : entry;
         }
+        // (a page that the sequence does not have has entry 0 and no valid token)
+        blk[0] = __builtin_amdgcn_readlane(entry, 2 * (i % (kWave / 2)));
+        blk[1] = __builtin_amdgcn_readlane(entry, 2 * (i % (kWave / 2)) + 1);
+    };
+    if (mine > 0) {
+        turn_to(0);
+        load_k<HD>(r, a, blk, kvh, lane);
+        load_v<HD>(r, a, blk, kvh, lane);
     }
+    stage_q<HD>(a.q + ((size_t)b * a.hq + h0) * HD, H, reinterpret_cast<_Float16*>(qops), qscale);
+    __syncthreads();
+    const h8_t* q = qops + lane;
+    const float scale = qscale[t & 7];
+    Fold<HD> f;
+#pragma unroll
+    for (int nt = 0; nt < HD / 16; ++nt) f.o[nt] = f4_t{0.f, 0.f, 0.f, 0.f};
+    auto use = [&](int i, auto next_k) {
+        const int page = 2 * (first + stride * i);
+        float* raw = ACC && t < H ? a.raw + ((size_t)b * a.hq + h0 + t) * cap + page * kPage + 4 * g : nullptr;
+        fold<HD, ACC>(f, r, q, scale, min(ctx - page * kPage, kPage), min(max(ctx - (page + 1) * kPage, 0), kPage), raw, lane, next_k);
+    };
+    // (the last pair apart: a request that may not come makes the waits for
+    // others wait for all)
+    for (int i = 0; i + 1 < mine; ++i) {
+        use(i, [&] {
+            turn_to(i + 1);
+            load_k<HD>(r, a, blk, kvh, lane);
+        });
+        load_v<HD>(r, a, blk, kvh, lane);
+    }
+    if (mine > 0) use(mine - 1, [] {});
+    const float factor = __builtin_amdgcn_exp2f(kUp - f.up);  // records have 2^kUp
+    float l = f.l * factor;
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     if constexpr (!INT4) {  // the low parts' rows
 #pragma unroll
         for (int nt = 0; nt < HD / 16; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[nt][j] += __shfl_xor(o[nt][j], 32, 64);
+            for (int j = 0; j < 4; ++j) f.o[nt][j] += __shfl_xor(f.o[nt][j], 32, 64);
     }
     // one record per wavefront in LDS: O[H][HD], M[H], L[H]
     const int rec = H * (HD + 2);
@@ -356,29 +443,29 @@ __global__ __launch_bounds__(kThreads) void k_attn(AttnArgs a) {
     for (int nt = 0; nt < HD / 16; ++nt)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (4 * g + j < H) my[(4 * g + j) * HD + 16 * nt + t] = o[nt][j];
+            if (4 * g + j < H) my[(4 * g + j) * HD + 16 * nt + t] = f.o[nt][j] * factor;
     if (g == 0 && t < H) {
         // M is NaN where the length or the table is out of range
-        my[H * HD + t] = bad ? __builtin_nanf("") : m;
+        my[H * HD + t] = bad ? __builtin_nanf("") : f.m;
         my[H * HD + H + t] = l;
     }
     __syncthreads();
     float* part = a.part + (((size_t)b * a.hkv * a.plan.groups + blockIdx.y) * a.plan.splits + split) * a.plan.rec;
     for (int x = threadIdx.x; x < H * HD; x += kThreads) {
         const int h = x / HD;
-        float M = -__builtin_inff(), acc = 0.0f, L = 0.0f;
+        float mw[kWaves], M = -__builtin_inff(), acc = 0.0f, L = 0.0f;
         bool no = false;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float mw = lds[w * rec + H * HD + h];
-            no = no || mw != mw;
-            M = fmaxf(M, mw);
+            mw[w] = lds[w * rec + H * HD + h];
+            no = no || mw[w] != mw[w];
+            M = fmaxf(M, mw[w]);
         }
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float f = M == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(lds[w * rec + H * HD + h] - M);
-            acc = fmaf(f, lds[w * rec + x], acc);
-            L = fmaf(f, lds[w * rec + H * HD + H + h], L);
+            const float e = M == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mw[w] - M);
+            acc = fmaf(e, lds[w * rec + x], acc);
+            L = fmaf(e, lds[w * rec + H * HD + H + h], L);
         }
         part[x] = acc;
         if (x % HD == 0) {
