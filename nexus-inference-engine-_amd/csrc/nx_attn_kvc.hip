@@ -43,6 +43,18 @@ constexpr int kRowRor8 = 0x128;
 constexpr float kUp = 15.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Lane l's and lane l ^ 16's (32's) larger value.
+__device__ inline float max_x16(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    const uint32_t x = a[0], y = a[1];
+    return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+__device__ inline float max_x32(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    const uint32_t x = a[0], y = a[1];
+    return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+
 // ------------------------------------------------------------------- pages --
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
@@ -273,42 +285,35 @@ __device__ inline void values(const PairF16<HD>& r, const float (&p)[8], f4_t (&
 // that low parts are normal fp16 numbers and no high part overflows; scale[t]
 // takes it back.
 template <int HD>
-__device__ inline void stage_q(const float* q, int H, _Float16* ops, float* scale) {
-    constexpr int T = HD / 4;  // threads of a head, four dimensions each
-    static_assert(T * kHeadsPerBlock <= kThreads && T <= kWave && kWave % T == 0, "a head lies in one wavefront");
-    const int h = threadIdx.x / T, d = 4 * (threadIdx.x % T);
-    if (h >= kHeadsPerBlock) return;
-    const f4_t x = h < H ? *reinterpret_cast<const f4_t*>(q + (size_t)h * HD + d) : f4_t{0.f, 0.f, 0.f, 0.f};
-    float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-    for (int o = 1; o < T; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
-    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
-    const int up = e == 0 || e == 255 ? 0 : min(136 - e, 126);
-    h4_t hi, lo;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float y = ldexpf(x[j], up);
-        hi[j] = (_Float16)y;
-        lo[j] = (_Float16)(y - (float)hi[j]);
+struct StageQ {
+    static constexpr int T = HD / 4;  // threads of a head, four dimensions each
+    static_assert(T * kHeadsPerBlock <= kThreads && kWave % T == 0, "a head lies in one wavefront");
+    f4_t x;
+    __device__ void request(const float* q, int H) {
+        const int h = threadIdx.x / T, d = 4 * (threadIdx.x % T);
+        x = h < H ? *reinterpret_cast<const f4_t*>(q + (size_t)h * HD + d) : f4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const int at = ((d / 32) * kWave + 16 * (d % 32 / 8)) * 8 + d % 8;
-    *reinterpret_cast<h4_t*>(ops + at + 8 * h) = hi;
-    *reinterpret_cast<h4_t*>(ops + at + 8 * (h + 8)) = lo;
-    if (d == 0) scale[h] = ldexpf(kLog2e / sqrtf((float)HD), -up);
-}
-
-// Maximum over the four lanes of a column (lanes l, l ^ 16, l ^ 32, l ^ 48).
-__device__ inline float column_max(float v) {
-    typedef uint32_t __attribute__((ext_vector_type(2))) pair_t;
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const pair_t a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t x0 = a[0], x1 = a[1];
-    const float m = fmaxf(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1));
-    const uint32_t w = __builtin_bit_cast(uint32_t, m);
-    const pair_t b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    const uint32_t y0 = b[0], y1 = b[1];
-    return fmaxf(__builtin_bit_cast(float, y0), __builtin_bit_cast(float, y1));
-}
+    __device__ void store(_Float16* ops, float* scale) const {
+        const int h = threadIdx.x / T, d = 4 * (threadIdx.x % T);
+        if (h >= kHeadsPerBlock) return;
+        float top = row16_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+        if (T >= 32) top = max_x16(top);
+        if (T >= 64) top = max_x32(top);
+        const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
+        const int up = e == 0 || e == 255 ? 0 : min(136 - e, 126);
+        h4_t hi, lo;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float y = ldexpf(x[j], up);
+            hi[j] = (_Float16)y;
+            lo[j] = (_Float16)(y - (float)hi[j]);
+        }
+        const int at = ((d / 32) * kWave + 16 * (d % 32 / 8)) * 8 + d % 8;
+        *reinterpret_cast<h4_t*>(ops + at + 8 * h) = hi;
+        *reinterpret_cast<h4_t*>(ops + at + 8 * (h + 8)) = lo;
+        if (d == 0) scale[h] = ldexpf(kLog2e / sqrtf((float)HD), -up);
+    }
+};
 
 // A pair of pages into the state.  The next pair's K is requested once this
 // one's has become scores, its V once this one's is added: half a pair is in
@@ -337,7 +342,7 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, float scale, in
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, p[j]);
-    top = column_max(top) * scale;
+    top = max_x32(max_x16(top)) * scale;  // over the column's four lanes
     const float mn = fmaxf(f.m, top);
     const bool none = mn == -__builtin_inff();  // no token, or NaN scores alone
     const float up = most_up<HD>(r, f.up);
@@ -366,7 +371,7 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, float scale, in
 }
 
 template <int HD, bool INT4, bool ACC>
-__global__ __launch_bounds__(kThreads, 2) void k_attn(AttnArgs a) {
+__global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void k_attn(AttnArgs a) {
     using Pair = typename std::conditional<INT4, PairI4<HD>, PairF16<HD>>::type;
     constexpr int kRec = kHeadsPerBlock * (HD + 2);
     __shared__ __align__(16) float lds[kWaves * kRec];
@@ -377,23 +382,31 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn(AttnArgs a) {
     const int split = blockIdx.x, kvh = blockIdx.y / a.plan.groups, grp = blockIdx.y % a.plan.groups, b = blockIdx.z;
     const int G = a.hq / a.hkv, H = min(kHeadsPerBlock, G - kHeadsPerBlock * grp), h0 = kvh * G + kHeadsPerBlock * grp;
     const int cap = a.max_blocks * kPage;
+    const int stride = a.plan.splits * kWaves, first = split + a.plan.splits * wave;
+    // q and the table entries of the first 32 pairs (two lanes each) are
+    // requested with the length, not behind it
+    StageQ<HD> stage;
+    stage.request(a.q + ((size_t)b * a.hq + h0) * HD, H);
+    const int32_t* table = a.table + (size_t)b * a.max_blocks;
+    auto entry_of = [&](int i) {
+        const int page = 2 * (first + stride * (i + lane / 2)) + (lane & 1);
+        return page < a.max_blocks ? table[page] : 0;
+    };
+    int entry = entry_of(0);
     int ctx = a.lens[b];
     bool bad = ctx < 0 || ctx > cap;
     ctx = bad ? 0 : ctx;
     const int npages = (ctx + kPage - 1) / kPage, npairs = (npages + 1) / 2;
-    const int stride = a.plan.splits * kWaves, first = split + a.plan.splits * wave;
     const int mine = first < npairs ? (npairs - first + stride - 1) / stride : 0;
-    const int32_t* table = a.table + (size_t)b * a.max_blocks;
-    int entry = 0, blk[2];
+    int blk[2];
     Pair r;
     // the pages of pair i of this wavefront, in order
     auto turn_to = [&](int i) {
-        if (i % (kWave / 2) == 0) {  // the table entries of the next 32 pairs, two lanes each
-            const int page = 2 * (first + stride * (i + lane / 2)) + (lane & 1);
-            entry = page < npages ? table[page] : 0;
-            const bool out = entry < 0 || entry >= a.num_blocks;
-            bad = bad || __any(out);
-            entry = out ? 0 : entry;
+        if (i % (kWave / 2) == 0) {
+            if (i > 0) entry = entry_of(i);
+            const bool used = 2 * (first + stride * (i + lane / 2)) + (lane & 1) < npages, out = entry < 0 || entry >= a.num_blocks;
+            bad = bad || __any(used && out);
+            entry = used && !out ? entry : 0;
         }
         // (a page that the sequence does not have has entry 0 and no valid token)
         blk[0] = __builtin_amdgcn_readlane(entry, 2 * (i % (kWave / 2)));
@@ -404,7 +417,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn(AttnArgs a) {
         load_k<HD>(r, a, blk, kvh, lane);
         load_v<HD>(r, a, blk, kvh, lane);
     }
-    stage_q<HD>(a.q + ((size_t)b * a.hq + h0) * HD, H, reinterpret_cast<_Float16*>(qops), qscale);
+    stage.store(reinterpret_cast<_Float16*>(qops), qscale);
     __syncthreads();
     const h8_t* q = qops + lane;
     const float scale = qscale[t & 7];
@@ -436,38 +449,40 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn(AttnArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) f.o[nt][j] += __shfl_xor(f.o[nt][j], 32, 64);
     }
-    // one record per wavefront in LDS: O[H][HD], M[H], L[H]
-    const int rec = H * (HD + 2);
-    float* my = lds + wave * rec;
+    // one record per wavefront in LDS: O[8][HD], M[8], L[8] (rows past H hold anything)
+    constexpr int MO = kHeadsPerBlock * HD, LO = MO + kHeadsPerBlock;
+    float* my = lds + wave * kRec;
+    if (g < 2) {
 #pragma unroll
-    for (int nt = 0; nt < HD / 16; ++nt)
+        for (int nt = 0; nt < HD / 16; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (4 * g + j < H) my[(4 * g + j) * HD + 16 * nt + t] = f.o[nt][j] * factor;
-    if (g == 0 && t < H) {
+            for (int j = 0; j < 4; ++j) my[(4 * g + j) * HD + 16 * nt + t] = f.o[nt][j] * factor;
+    }
+    if (lane < kHeadsPerBlock) {
         // M is NaN where the length or the table is out of range
-        my[H * HD + t] = bad ? __builtin_nanf("") : f.m;
-        my[H * HD + H + t] = l;
+        my[MO + lane] = bad ? __builtin_nanf("") : f.m;
+        my[LO + lane] = l;
     }
     __syncthreads();
     float* part = a.part + (((size_t)b * a.hkv * a.plan.groups + blockIdx.y) * a.plan.splits + split) * a.plan.rec;
-    for (int x = threadIdx.x; x < H * HD; x += kThreads) {
+    for (int x = 4 * threadIdx.x; x < H * HD; x += 4 * kThreads) {
         const int h = x / HD;
-        float mw[kWaves], M = -__builtin_inff(), acc = 0.0f, L = 0.0f;
+        float mw[kWaves], M = -__builtin_inff(), L = 0.0f;
         bool no = false;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            mw[w] = lds[w * rec + H * HD + h];
+            mw[w] = lds[w * kRec + MO + h];
             no = no || mw[w] != mw[w];
             M = fmaxf(M, mw[w]);
         }
+        f4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             const float e = M == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mw[w] - M);
-            acc = fmaf(e, lds[w * rec + x], acc);
-            L = fmaf(e, lds[w * rec + H * HD + H + h], L);
+            acc += e * *reinterpret_cast<const f4_t*>(lds + w * kRec + x);
+            L = fmaf(e, lds[w * kRec + LO + h], L);
         }
-        part[x] = acc;
+        *reinterpret_cast<f4_t*>(part + x) = acc;
         if (x % HD == 0) {
             part[a.plan.heads * HD + h] = no ? __builtin_nanf("") : M;
             part[a.plan.heads * HD + a.plan.heads + h] = L;
@@ -475,53 +490,77 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn(AttnArgs a) {
     }
 }
 
+// Blocks of a kernel that a compute unit holds at once.
+template <int HD, bool INT4, bool ACC>
+int blocks_per_cu() {
+    static int n = 0;
+    if (n == 0) {
+        int v = 0;
+        n = hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, k_attn<HD, INT4, ACC>, kThreads, 0) == hipSuccess && v > 0 ? v : 1;
+    }
+    return n;
+}
+
 // ------------------------------------------------------------------- k_join --
-// Block (j, kv head, sequence): the j-th share of the kv head's output and, with
-// weights, of its slots.
+// Block (j, kv head, sequence): `cols` float4 columns of the kv head's output,
+// their splits shared by the block's threads, and, with weights, every
+// gridDim.x-th 256 slots.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinHeads = 64;  // query heads of a kv head
 
 template <int HD, bool ACC>
-__global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int cols) {
     __shared__ float fac[kJoinHeads * kMaxSplits], top[kJoinHeads], inv[kJoinHeads];
+    __shared__ f4_t sums[kJoinThreads];
     __shared__ int refused;
-    const int kvh = blockIdx.y, b = blockIdx.z, G = a.hq / a.hkv, ns = a.plan.splits, tid = threadIdx.x;
-    const float* parts = a.part + ((size_t)b * a.hkv + kvh) * a.plan.groups * ns * a.plan.rec;
+    const int kvh = blockIdx.y, b = blockIdx.z, G = a.hq / a.hkv, ns = a.plan.splits, tid = threadIdx.x, rec = a.plan.rec;
+    const float* parts = a.part + ((size_t)b * a.hkv + kvh) * a.plan.groups * ns * rec;
+    const int total = G * HD / 4, col = blockIdx.x * cols + tid % cols, s0 = tid / cols, step = kJoinThreads / cols;
+    const bool mine = (int)blockIdx.x * cols < total;  // the block has output
     if (tid == 0) refused = 0;
     __syncthreads();
     // wavefront w: heads w, w + 4, ..; lane s: split s
-    const int lane = tid & 63;
-    for (int h = tid / kWave; h < G; h += kJoinThreads / kWave) {
-        const float* p = parts + ((size_t)(h / kHeadsPerBlock) * ns + min(lane, ns - 1)) * a.plan.rec + a.plan.heads * HD + h % kHeadsPerBlock;
-        const float m = lane < ns ? p[0] : -__builtin_inff(), l = lane < ns ? p[a.plan.heads] : 0.0f;
-        const float M = wave_max(m);
-        const bool none = M == -__builtin_inff();
-        const float e = none ? 1.0f : __builtin_amdgcn_exp2f(m - M), L = wave_sum(e * l);
-        const bool no = __any(m != m);
-        const float il = no ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
-        if (lane < ns) fac[h * kMaxSplits + lane] = no ? il : e * il;
-        if (lane == 0) {
-            top[h] = M - kUp;
-            inv[h] = il;
-            if (no) refused = 1;
+    const int lane = tid & 63, slane = min(lane, ns - 1);
+    for (int h0 = tid / kWave; h0 < G; h0 += 4 * kJoinThreads / kWave) {
+        float m[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int h = min(h0 + i * kJoinThreads / kWave, G - 1);
+            const float* p = parts + ((size_t)(h / kHeadsPerBlock) * ns + slane) * rec + a.plan.heads * HD + h % kHeadsPerBlock;
+            m[i] = p[0];
+            l[i] = p[a.plan.heads];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int h = h0 + i * kJoinThreads / kWave;
+            if (h >= G) break;
+            const float M = wave_max(m[i]);  // (past the last split: that one again)
+            const bool none = M == -__builtin_inff();
+            const float e = lane >= ns ? 0.0f : none ? 1.0f : __builtin_amdgcn_exp2f(m[i] - M), L = wave_sum(lane < ns ? e * l[i] : 0.0f);
+            const bool no = __any(m[i] != m[i]);
+            const float il = no ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
+            if (lane < ns) fac[h * kMaxSplits + lane] = no ? il : e * il;
+            if (lane == 0) {
+                top[h] = M - kUp;
+                inv[h] = il;
+                if (no) refused = 1;
+            }
         }
     }
     __syncthreads();
-    const int total = G * HD, per = ((total + (int)gridDim.x - 1) / (int)gridDim.x + 3) / 4 * 4;
-    uint16_t* out = a.out + ((size_t)b * a.hq + (size_t)kvh * G) * HD;
-    const int end = min(total, (int)(blockIdx.x + 1) * per);
-    for (int x = (int)blockIdx.x * per + 4 * tid; x < end; x += 4 * kJoinThreads) {
-        const int h = x / HD;
-        const float* p = parts + (size_t)(h / kHeadsPerBlock) * ns * a.plan.rec + (h % kHeadsPerBlock) * HD + x % HD;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mine) {
+        const int c = min(col, total - 1), h = 4 * c / HD;
+        const float* p = parts + (size_t)(h / kHeadsPerBlock) * ns * rec + (h % kHeadsPerBlock) * HD + 4 * c % HD;
+        f4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-        for (int s = 0; s < ns; ++s) {
-            const float4 v = *reinterpret_cast<const float4*>(p + (size_t)s * a.plan.rec);
-            const float f = fac[h * kMaxSplits + s];
-            acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+        for (int s = s0; s < ns; s += step) acc += fac[h * kMaxSplits + s] * *reinterpret_cast<const f4_t*>(p + (size_t)s * rec);
+        sums[tid] = acc;
+        __syncthreads();
+        if (tid < cols && col < total) {
+            for (int i = 1; i < min(step, ns); ++i) acc += sums[i * cols + tid];
+            *reinterpret_cast<uint2*>(a.out + ((size_t)b * a.hq + (size_t)kvh * G) * HD + 4 * col) =
+                make_uint2((uint32_t)f2h_bits(acc[0]) | ((uint32_t)f2h_bits(acc[1]) << 16), (uint32_t)f2h_bits(acc[2]) | ((uint32_t)f2h_bits(acc[3]) << 16));
         }
-        *reinterpret_cast<uint2*>(out + x) = make_uint2((uint32_t)f2h_bits(acc.x) | ((uint32_t)f2h_bits(acc.y) << 16),
-                                                        (uint32_t)f2h_bits(acc.z) | ((uint32_t)f2h_bits(acc.w) << 16));
     }
     if constexpr (ACC) {
         if (refused) return;
@@ -530,6 +569,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a) {
         const float* raw = a.raw + ((size_t)b * a.hq + (size_t)kvh * G) * cap;
         for (int s = (int)blockIdx.x * kJoinThreads + tid; s < ctx; s += (int)gridDim.x * kJoinThreads) {
             float acc = 0.0f;
+#pragma unroll 8
             for (int h = 0; h < G; ++h) acc = fmaf(__builtin_amdgcn_exp2f(raw[(size_t)h * cap + s] - top[h]), inv[h], acc);
             w[s] += acc;
         }
@@ -539,31 +579,43 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a) {
 template <int HD, bool INT4>
 hipError_t attn_case(const AttnArgs& a, hipStream_t st) {
     const dim3 grid(a.plan.splits, a.hkv * a.plan.groups, a.batch);
-    const int slots = a.max_blocks * kPage;
-    if (a.weights) {
-        hipLaunchKernelGGL((k_attn<HD, INT4, true>), grid, dim3(kThreads), 0, st, a);
-        const unsigned n = (unsigned)std::min(64, std::max(1, slots / (2 * kJoinThreads)));
-        hipLaunchKernelGGL((k_join<HD, true>), dim3(n, a.hkv, a.batch), dim3(kJoinThreads), 0, st, a);
-    } else {
-        hipLaunchKernelGGL((k_attn<HD, INT4, false>), grid, dim3(kThreads), 0, st, a);
-        const unsigned n = (unsigned)std::max(1, a.hq / a.hkv * HD / 128);
-        hipLaunchKernelGGL((k_join<HD, false>), dim3(n, a.hkv, a.batch), dim3(kJoinThreads), 0, st, a);
+    const int total = a.hq / a.hkv * HD / 4;
+    // 32 columns to a block, eight threads to a column; with weights as many
+    // blocks as there are 256 slots, up to 128, and at least 8 columns to one
+    int n = (total + 31) / 32, cols = 32;
+    if constexpr (INT4) {  // (fp16 pages without weights are nx_attn.hip's)
+        if (!a.weights) {
+            hipLaunchKernelGGL((k_attn<HD, true, false>), grid, dim3(kThreads), 0, st, a);
+            hipLaunchKernelGGL((k_join<HD, false>), dim3(n, a.hkv, a.batch), dim3(kJoinThreads), 0, st, a, cols);
+            return hipGetLastError();
+        }
     }
+    n = std::max(n, std::min(128, (a.max_blocks * kPage + kJoinThreads - 1) / kJoinThreads));
+    while (cols > 8 && n * cols / 2 >= total) cols /= 2;
+    hipLaunchKernelGGL((k_attn<HD, INT4, true>), grid, dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((k_join<HD, true>), dim3(n, a.hkv, a.batch), dim3(kJoinThreads), 0, st, a, cols);
     return hipGetLastError();
+}
+
+template <bool INT4, bool ACC>
+int held(int hd) {
+    return hd == 64 ? blocks_per_cu<64, INT4, ACC>() : hd == 128 ? blocks_per_cu<128, INT4, ACC>() : blocks_per_cu<256, INT4, ACC>();
 }
 
 }  // namespace
 
-AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks) {
+AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4, bool weights) {
     AttnPlan p;
     const int G = hq / hkv, pairs = (max_blocks + 1) / 2;
     p.groups = (G + kHeadsPerBlock - 1) / kHeadsPerBlock;
     p.heads = std::min(G, kHeadsPerBlock);
     p.rec = (p.heads * (hd + 2) + 3) / 4 * 4;
-    // two blocks to a compute unit, and a pair of pages at least to a wavefront
+    // as many blocks as the device holds at once (a second round of them would
+    // begin when the first is done: 27 against PLAN_US us for 8 fp16 sequences of
+    // 4K), and a pair of pages at least to a wavefront
     const int64_t rows = (int64_t)batch * hkv * p.groups;
-    const int64_t want = (2 * (int64_t)device_cus() + rows - 1) / rows;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (pairs + kWaves - 1) / kWaves, kMaxSplits}));
+    const int64_t room = (int64_t)device_cus() * (int4 ? weights ? held<true, true>(hd) : held<true, false>(hd) : held<false, true>(hd));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({room / rows, (pairs + kWaves - 1) / kWaves, kMaxSplits}));
     return p;
 }
 

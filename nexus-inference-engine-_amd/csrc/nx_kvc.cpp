@@ -129,7 +129,7 @@ nx_status attn_kvc(nx_ctx* ctx, const char* name, bool int4, nx_buf q, nx_buf kp
     nx::kvc::AttnArgs a{};
     if (ctx->device < 0) return fail(ctx, NX_ERR_NO_DEVICE, "%s: no device", name);
     const OnDevice on(ctx->device);
-    a.plan = nx::kvc::attn_plan(batch, hq, hkv, hd, max_blocks);
+    a.plan = nx::kvc::attn_plan(batch, hq, hkv, hd, max_blocks, int4, weights != 0);
     s = kvc_ws(ctx, attn_ws_bytes(a.plan, batch, hq, hkv, max_blocks, weights != 0), name);
     if (s != NX_OK) return s;
     a.q = dptr<const float>(q);
@@ -211,7 +211,8 @@ nx_status kvc_reserve(nx_ctx* ctx, int batch, int hq, int hkv, int hd, int max_c
     size_t bytes = 4 * kvc::evict_ws_words(batch, hkv, blocks, blocks * kPage);
     // (a smaller batch may split its pages further)
     for (int b = 1; b <= batch; ++b)
-        bytes = std::max(bytes, attn_ws_bytes(kvc::attn_plan(b, hq, hkv, hd, blocks), b, hq, hkv, blocks, true));
+        for (bool int4 : {false, true})
+            bytes = std::max(bytes, attn_ws_bytes(kvc::attn_plan(b, hq, hkv, hd, blocks, int4, true), b, hq, hkv, blocks, true));
     return kvc_ws(ctx, bytes, "nx_reserve_workspace");
 }
 }  // namespace nx

@@ -64,7 +64,7 @@ struct AttnPlan {
     int splits;  // blocks that share the pages of one (sequence, kv head)
     int rec;     // floats of a record: O[heads][hd], M[heads], L[heads]
 };
-AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks);
+AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4, bool weights);
 
 struct AttnArgs {
     const float* q;          // [batch][hq][hd]
