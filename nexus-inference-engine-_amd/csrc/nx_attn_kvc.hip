@@ -1,15 +1,17 @@
 // Decode attention over int4-g32 pages, and over fp16 pages with the weight
 // of every cached token added to an array.
 //
-// Two launches.  k_attn: a block of 8 wavefronts takes every splits-th pair of
-// pages of one kv head for up to 8 of its query heads, keeps an online softmax
-// per head, merges its wavefronts through LDS and writes one record (O, M, L);
-// with weights it also writes the scores.  k_join: blocks share the merge of
-// the records into the fp16 output and, with weights, turn the scores into
-// exp(s - M) / L and add their sum over the query heads of the kv head.  (The
-// scores need M and L of all splits, which no block of k_attn has; reading
-// them back costs 8 bytes a token and query head, the pages again would cost 9/16
-// byte or more a value.)
+// k_attn: a block of 8 wavefronts takes every splits-th pair of pages of one
+// kv head for up to 8 of its query heads, keeps an online softmax per head,
+// merges its wavefronts through LDS and writes one record (O, M, L), or the
+// fp16 output where it has the kv head to itself.  With weights it also writes
+// the scores.  k_join: merges the records and, with weights, turns the scores
+// into exp(s - M) / L, whose sum over the query heads of the kv head it adds to
+// the weights.  (The scores need M and L of all splits, which no block of k_attn
+// has; reading them back costs 8 bytes a token and query head, the pages again
+// would cost 9/16 byte or more a value.  Merging the records in the last block of
+// k_attn instead took as long for 8 splits and longer for more: 18.3 against
+// 15.5 us for 64.)
 //
 // Products are v_mfma_f32_16x16x32_f16 (A: lane l holds row l%16, k = 8 (l/16)
 // .. +7; B: column l%16, the same k; C: column l%16, rows 4 (l/16) .. +3).
@@ -40,7 +42,7 @@ constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kMaxSplits = 64;
 constexpr int kRowRor8 = 0x128;
-constexpr float kUp = 15.0f;
+constexpr float kUp = 11.0f, kLead = 4.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Lane l's and lane l ^ 16's (32's) larger value.
@@ -209,10 +211,13 @@ __device__ inline void clear_past(PairF16<HD>& r, int na, int nb, int lane) {
         for (int nt = 0; nt < HD / 16; ++nt) r.v[nt][pg] &= u2_t{m[pg].x, m[pg].y};
 }
 
-// One wavefront's state over its pairs of pages: a column's running maximum (of
+// One wavefront's state over its pairs of pages: a column's reference m (of
 // scores times log2 e), this lane's part of its sum, and O.  Probabilities are
-// exp2(s - max + up), up to 2^15 instead of 1, so that small ones stay normal
+// exp2(s - m + up), up to 2^15 instead of 1, so that small ones stay normal
 // fp16 numbers (below 2^-14 fp16 loses bits); L and O have the same factor.
+// The reference is the first pair's maximum and follows a larger one only when
+// that is more than 2^kLead ahead (kUp + kLead is 15): O is hardly ever
+// multiplied through.
 template <int HD>
 struct Fold {
     float m = -__builtin_inff(), l = 0.0f, up = kUp;
@@ -220,7 +225,7 @@ struct Fold {
 };
 
 // ------------------------------------------------------------ values of a pair --
-// The powers of two that the probabilities of a pair may have.  P V takes p
+// The powers of two that a pair's probabilities may have.  P V takes p
 // times the token's scale, rounded to fp16: at most 2^-11 of a term, which
 // stays linear in the output (an fp16 number itself).  With p up to 2^15 a
 // scale of 2 or more (a value of 16 and up among a group) could pass the
@@ -239,7 +244,8 @@ __device__ inline float most_up(const PairI4<HD>& r, float up) {
             most = __builtin_elementwise_max(most, __builtin_elementwise_max(__builtin_shufflevector(w, w, 0, 1), __builtin_shufflevector(w, w, 2, 3)));
         }
     const int e = max((int)most.x, (int)most.y) >> 10;  // biased exponent: 15 is 2^0
-    return __any(e > 30 - (int)up) ? 30.0f - wave_max((float)e) : up;
+    constexpr int kTop = 15 + (int)kUp;
+    return __any(e > kTop - (int)up) ? (float)kTop - wave_max((float)e) : up;
 }
 template <int HD>
 __device__ inline float most_up(const PairF16<HD>&, float up) {
@@ -343,7 +349,7 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, float scale, in
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, p[j]);
     top = max_x32(max_x16(top)) * scale;  // over the column's four lanes
-    const float mn = fmaxf(f.m, top);
+    const float mn = top > f.m + kLead ? top : f.m;
     const bool none = mn == -__builtin_inff();  // no token, or NaN scores alone
     const float up = most_up<HD>(r, f.up);
     const float corr = none ? 1.0f : __builtin_amdgcn_exp2f(f.m - mn + (up - f.up)), from = none ? 0.0f : mn - up;
@@ -368,6 +374,11 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, float scale, in
     f.m = mn;
     f.up = up;
     values<HD>(r, p, f.o, lane);
+}
+
+__device__ inline void store_out(uint16_t* out, f4_t v) {
+    *reinterpret_cast<uint2*>(out) =
+        make_uint2((uint32_t)f2h_bits(v[0]) | ((uint32_t)f2h_bits(v[1]) << 16), (uint32_t)f2h_bits(v[2]) | ((uint32_t)f2h_bits(v[3]) << 16));
 }
 
 template <int HD, bool INT4, bool ACC>
@@ -464,7 +475,10 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
         my[LO + lane] = l;
     }
     __syncthreads();
-    float* part = a.part + (((size_t)b * a.hkv * a.plan.groups + blockIdx.y) * a.plan.splits + split) * a.plan.rec;
+    const size_t row = (size_t)b * a.hkv * a.plan.groups + blockIdx.y;
+    float* part = a.part + (row * a.plan.splits + split) * a.plan.rec;
+    const int MP = a.plan.heads * HD, LP = MP + a.plan.heads;  // of a record in memory
+    uint16_t* out = a.out + ((size_t)b * a.hq + h0) * HD;
     for (int x = 4 * threadIdx.x; x < H * HD; x += 4 * kThreads) {
         const int h = x / HD;
         float mw[kWaves], M = -__builtin_inff(), L = 0.0f;
@@ -482,10 +496,15 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
             acc += e * *reinterpret_cast<const f4_t*>(lds + w * kRec + x);
             L = fmaf(e, lds[w * kRec + LO + h], L);
         }
-        *reinterpret_cast<f4_t*>(part + x) = acc;
-        if (x % HD == 0) {
-            part[a.plan.heads * HD + h] = no ? __builtin_nanf("") : M;
-            part[a.plan.heads * HD + a.plan.heads + h] = L;
+        if (a.plan.join) {
+            *reinterpret_cast<f4_t*>(part + x) = acc;
+            if (x % HD == 0) {
+                part[MP + h] = no ? __builtin_nanf("") : M;
+                part[LP + h] = L;
+            }
+        } else {  // the one block of its kv head
+            const float il = no ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
+            store_out(out + x, acc * il);
         }
     }
 }
@@ -502,21 +521,31 @@ int blocks_per_cu() {
 }
 
 // ------------------------------------------------------------------- k_join --
-// Block (j, kv head, sequence): `cols` float4 columns of the kv head's output,
-// their splits shared by the block's threads, and, with weights, every
-// gridDim.x-th 256 slots.
-constexpr int kJoinThreads = 256;
+// With weights.  The first `outs` blocks of a (kv head, sequence) merge the
+// records into 32 float4 columns of the output each, eight threads to a column;
+// the others turn 256 slots' scores into weights at a time.
+constexpr int kJoinThreads = 256, kJoinCols = 32;
 constexpr int kJoinHeads = 64;  // query heads of a kv head
 
-template <int HD, bool ACC>
-__global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int cols) {
+template <int HD>
+__global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int outs) {
     __shared__ float fac[kJoinHeads * kMaxSplits], top[kJoinHeads], inv[kJoinHeads];
     __shared__ f4_t sums[kJoinThreads];
     __shared__ int refused;
     const int kvh = blockIdx.y, b = blockIdx.z, G = a.hq / a.hkv, ns = a.plan.splits, tid = threadIdx.x, rec = a.plan.rec;
     const float* parts = a.part + ((size_t)b * a.hkv + kvh) * a.plan.groups * ns * rec;
-    const int total = G * HD / 4, col = blockIdx.x * cols + tid % cols, s0 = tid / cols, step = kJoinThreads / cols;
-    const bool mine = (int)blockIdx.x * cols < total;  // the block has output
+    const bool output = (int)blockIdx.x < outs;
+    // the thread's first slot's scores and weight are requested ahead of all else
+    const int cap = a.max_blocks * kPage, slot = ((int)blockIdx.x - outs) * kJoinThreads + tid;
+    const float* raw = a.raw + ((size_t)b * a.hq + (size_t)kvh * G) * cap;
+    float* weights = a.weights + ((size_t)b * a.hkv + kvh) * cap;
+    float early[8], was = 0.0f;
+    if (!output) {
+        const int s = min(slot, cap - 1);
+#pragma unroll
+        for (int h = 0; h < 8; ++h) early[h] = raw[(size_t)min(h, G - 1) * cap + s];
+        was = weights[s];
+    }
     if (tid == 0) refused = 0;
     __syncthreads();
     // wavefront w: heads w, w + 4, ..; lane s: split s
@@ -535,8 +564,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int cols) {
             const int h = h0 + i * kJoinThreads / kWave;
             if (h >= G) break;
             const float M = wave_max(m[i]);  // (past the last split: that one again)
-            const bool none = M == -__builtin_inff();
-            const float e = lane >= ns ? 0.0f : none ? 1.0f : __builtin_amdgcn_exp2f(m[i] - M), L = wave_sum(lane < ns ? e * l[i] : 0.0f);
+            const float e = lane >= ns ? 0.0f : M == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[i] - M), L = wave_sum(lane < ns ? e * l[i] : 0.0f);
             const bool no = __any(m[i] != m[i]);
             const float il = no ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
             if (lane < ns) fac[h * kMaxSplits + lane] = no ? il : e * il;
@@ -548,52 +576,51 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int cols) {
         }
     }
     __syncthreads();
-    if (mine) {
+    if (output) {
+        const int total = G * HD / 4, col = blockIdx.x * kJoinCols + tid % kJoinCols, step = kJoinThreads / kJoinCols;
         const int c = min(col, total - 1), h = 4 * c / HD;
         const float* p = parts + (size_t)(h / kHeadsPerBlock) * ns * rec + (h % kHeadsPerBlock) * HD + 4 * c % HD;
         f4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-        for (int s = s0; s < ns; s += step) acc += fac[h * kMaxSplits + s] * *reinterpret_cast<const f4_t*>(p + (size_t)s * rec);
+        for (int s = tid / kJoinCols; s < ns; s += step) acc += fac[h * kMaxSplits + s] * *reinterpret_cast<const f4_t*>(p + (size_t)s * rec);
         sums[tid] = acc;
         __syncthreads();
-        if (tid < cols && col < total) {
-            for (int i = 1; i < min(step, ns); ++i) acc += sums[i * cols + tid];
-            *reinterpret_cast<uint2*>(a.out + ((size_t)b * a.hq + (size_t)kvh * G) * HD + 4 * col) =
-                make_uint2((uint32_t)f2h_bits(acc[0]) | ((uint32_t)f2h_bits(acc[1]) << 16), (uint32_t)f2h_bits(acc[2]) | ((uint32_t)f2h_bits(acc[3]) << 16));
+        if (tid < kJoinCols && col < total) {
+            for (int i = 1; i < step; ++i) acc += sums[i * kJoinCols + tid];
+            store_out(a.out + ((size_t)b * a.hq + (size_t)kvh * G) * HD + 4 * col, acc);
         }
+        return;
     }
-    if constexpr (ACC) {
-        if (refused) return;
-        const int cap = a.max_blocks * kPage, ctx = a.lens[b];
-        float* w = a.weights + ((size_t)b * a.hkv + kvh) * cap;
-        const float* raw = a.raw + ((size_t)b * a.hq + (size_t)kvh * G) * cap;
-        for (int s = (int)blockIdx.x * kJoinThreads + tid; s < ctx; s += (int)gridDim.x * kJoinThreads) {
-            float acc = 0.0f;
+    if (refused) return;
+    const int ctx = a.lens[b], stride = ((int)gridDim.x - outs) * kJoinThreads;
+    auto part_of = [&](float x, int h) { return __builtin_amdgcn_exp2f(x - top[h]) * inv[h]; };
+    if (slot < ctx) {
+        float acc = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 8; ++h)
+            if (h < G) acc += part_of(early[h], h);
+        for (int h = 8; h < G; ++h) acc += part_of(raw[(size_t)h * cap + slot], h);
+        weights[slot] = was + acc;
+    }
+    for (int64_t s = (int64_t)slot + stride; s < ctx; s += stride) {
+        float acc = 0.0f;
 #pragma unroll 8
-            for (int h = 0; h < G; ++h) acc = fmaf(__builtin_amdgcn_exp2f(raw[(size_t)h * cap + s] - top[h]), inv[h], acc);
-            w[s] += acc;
-        }
+        for (int h = 0; h < G; ++h) acc += part_of(raw[(size_t)h * cap + s], h);
+        weights[s] += acc;
     }
 }
 
 template <int HD, bool INT4>
 hipError_t attn_case(const AttnArgs& a, hipStream_t st) {
     const dim3 grid(a.plan.splits, a.hkv * a.plan.groups, a.batch);
-    const int total = a.hq / a.hkv * HD / 4;
-    // 32 columns to a block, eight threads to a column; with weights as many
-    // blocks as there are 256 slots, up to 128, and at least 8 columns to one
-    int n = (total + 31) / 32, cols = 32;
-    if constexpr (INT4) {  // (fp16 pages without weights are nx_attn.hip's)
-        if (!a.weights) {
-            hipLaunchKernelGGL((k_attn<HD, true, false>), grid, dim3(kThreads), 0, st, a);
-            hipLaunchKernelGGL((k_join<HD, false>), dim3(n, a.hkv, a.batch), dim3(kJoinThreads), 0, st, a, cols);
-            return hipGetLastError();
-        }
-    }
-    n = std::max(n, std::min(128, (a.max_blocks * kPage + kJoinThreads - 1) / kJoinThreads));
-    while (cols > 8 && n * cols / 2 >= total) cols /= 2;
-    hipLaunchKernelGGL((k_attn<HD, INT4, true>), grid, dim3(kThreads), 0, st, a);
-    hipLaunchKernelGGL((k_join<HD, true>), dim3(n, a.hkv, a.batch), dim3(kJoinThreads), 0, st, a, cols);
+    if (a.weights)
+        hipLaunchKernelGGL((k_attn<HD, INT4, true>), grid, dim3(kThreads), 0, st, a);
+    else if constexpr (INT4)  // (fp16 pages without weights are nx_attn.hip's)
+        hipLaunchKernelGGL((k_attn<HD, true, false>), grid, dim3(kThreads), 0, st, a);
+    if (!a.plan.join) return hipGetLastError();
+    const int outs = (a.hq / a.hkv * HD / 4 + kJoinCols - 1) / kJoinCols;
+    const int slots = a.weights ? std::min(128, (a.max_blocks * kPage + kJoinThreads - 1) / kJoinThreads) : 0;
+    hipLaunchKernelGGL(k_join<HD>, dim3(outs + slots, a.hkv, a.batch), dim3(kJoinThreads), 0, st, a, outs);
     return hipGetLastError();
 }
 
@@ -611,11 +638,12 @@ AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4
     p.heads = std::min(G, kHeadsPerBlock);
     p.rec = (p.heads * (hd + 2) + 3) / 4 * 4;
     // as many blocks as the device holds at once (a second round of them would
-    // begin when the first is done: 27 against PLAN_US us for 8 fp16 sequences of
+    // begin when the first is done: 27.5 against 26 us for 8 fp16 sequences of
     // 4K), and a pair of pages at least to a wavefront
     const int64_t rows = (int64_t)batch * hkv * p.groups;
     const int64_t room = (int64_t)device_cus() * (int4 ? weights ? held<true, true>(hd) : held<true, false>(hd) : held<false, true>(hd));
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({room / rows, (pairs + kWaves - 1) / kWaves, kMaxSplits}));
+    p.join = weights || p.splits > 1;
     return p;
 }
 

@@ -63,6 +63,7 @@ struct AttnPlan {
     int heads;   // query heads of a block's record
     int splits;  // blocks that share the pages of one (sequence, kv head)
     int rec;     // floats of a record: O[heads][hd], M[heads], L[heads]
+    bool join;   // a second launch merges the records
 };
 AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4, bool weights);
 

@@ -778,15 +778,16 @@ def test_workspace_grows_inside_a_token_batch():
                 kp, vp, _, _, table = cache(rng, True, [n] * B, 2, 64, mb, B * mb, stale=0.0)
                 cases.append((Held(c, q=rng.normal(0, 1, (B, 8, 64)).astype(np.float32), kp=kp, vp=vp, table=table,
                                    lens=np.array([n] * B, np.int32), out=np.zeros((B, 8, 64), np.float16),
-                                   w=np.zeros((B, 2, mb * PAGE), np.float32)), B, mb))
+                                   plain=np.zeros((B, 8, 64), np.float16), w=np.zeros((B, 2, mb * PAGE), np.float32)), B, mb))
             if capture:
                 c.check(c.L.nx_token_begin(c.h), "begin")
             for h, B, mb in cases:
+                c.attn_decode_paged_int4(h["q"], h["kp"], h["vp"], h["table"], h["lens"], h["plain"], 0, B, 8, 2, 64, mb, B * mb)
                 c.attn_decode_paged_int4(h["q"], h["kp"], h["vp"], h["table"], h["lens"], h["out"], h["w"], B, 8, 2, 64, mb, B * mb)
             if capture:
                 c.check(c.L.nx_token_end(c.h), "end")
             for h, _, _ in cases:
-                got += [h.get("out"), h.get("w")]
+                got += [h.get("out"), h.get("w"), h.get("plain")]
             return got
 
     want = outputs(False, False)
