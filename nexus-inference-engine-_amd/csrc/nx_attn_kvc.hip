@@ -45,11 +45,21 @@ constexpr int kRowRor8 = 0x128;
 constexpr float kUp = 11.0f, kLead = 4.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Lane l's and lane l ^ 16's (32's) larger value.
+// Lane l's and lane l ^ 16's (32's) larger value, and their sum.
 __device__ inline float max_x16(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
     const uint32_t x = a[0], y = a[1];
     return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+__device__ inline float sum_x16(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    const uint32_t x = a[0], y = a[1];
+    return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+}
+__device__ inline float sum_x32(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    const uint32_t x = a[0], y = a[1];
+    return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
 }
 __device__ inline float max_x32(float v) {
     const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
@@ -426,10 +436,10 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
     if (mine > 0) {
         turn_to(0);
         load_k<HD>(r, a, blk, kvh, lane);
-        load_v<HD>(r, a, blk, kvh, lane);
     }
     stage.store(reinterpret_cast<_Float16*>(qops), qscale);
     __syncthreads();
+    if (mine > 0) load_v<HD>(r, a, blk, kvh, lane);
     const h8_t* q = qops + lane;
     const float scale = qscale[t & 7];
     Fold<HD> f;
@@ -451,14 +461,12 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
     }
     if (mine > 0) use(mine - 1, [] {});
     const float factor = __builtin_amdgcn_exp2f(kUp - f.up);  // records have 2^kUp
-    float l = f.l * factor;
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    const float l = sum_x32(sum_x16(f.l)) * factor;
     if constexpr (!INT4) {  // the low parts' rows
 #pragma unroll
         for (int nt = 0; nt < HD / 16; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f.o[nt][j] += __shfl_xor(f.o[nt][j], 32, 64);
+            for (int j = 0; j < 4; ++j) f.o[nt][j] = sum_x32(f.o[nt][j]);
     }
     // one record per wavefront in LDS: O[8][HD], M[8], L[8] (rows past H hold anything)
     constexpr int MO = kHeadsPerBlock * HD, LO = MO + kHeadsPerBlock;
@@ -539,8 +547,16 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int outs) {
     const int cap = a.max_blocks * kPage, slot = ((int)blockIdx.x - outs) * kJoinThreads + tid;
     const float* raw = a.raw + ((size_t)b * a.hq + (size_t)kvh * G) * cap;
     float* weights = a.weights + ((size_t)b * a.hkv + kvh) * cap;
+    // (an output block's: its first eight splits' columns)
+    const int total = G * HD / 4, col = blockIdx.x * kJoinCols + tid % kJoinCols, c = min(col, total - 1), split0 = tid / kJoinCols;
+    constexpr int step = kJoinThreads / kJoinCols, kAhead = 8;
+    const float* column = parts + (size_t)(4 * c / HD / kHeadsPerBlock) * ns * rec + 4 * c % (kHeadsPerBlock * HD);
     float early[8], was = 0.0f;
-    if (!output) {
+    f4_t v[kAhead];
+    if (output) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) v[u] = *reinterpret_cast<const f4_t*>(column + (size_t)min(split0 + u * step, ns - 1) * rec);
+    } else {
         const int s = min(slot, cap - 1);
 #pragma unroll
         for (int h = 0; h < 8; ++h) early[h] = raw[(size_t)min(h, G - 1) * cap + s];
@@ -577,12 +593,12 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int outs) {
     }
     __syncthreads();
     if (output) {
-        const int total = G * HD / 4, col = blockIdx.x * kJoinCols + tid % kJoinCols, step = kJoinThreads / kJoinCols;
-        const int c = min(col, total - 1), h = 4 * c / HD;
-        const float* p = parts + (size_t)(h / kHeadsPerBlock) * ns * rec + (h % kHeadsPerBlock) * HD + 4 * c % HD;
+        static_assert(kAhead * step >= kMaxSplits, "all of a column's splits");
+        const int h = 4 * c / HD;
         f4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int s = tid / kJoinCols; s < ns; s += step) acc += fac[h * kMaxSplits + s] * *reinterpret_cast<const f4_t*>(p + (size_t)s * rec);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (split0 + u * step < ns) acc += fac[h * kMaxSplits + split0 + u * step] * v[u];
         sums[tid] = acc;
         __syncthreads();
         if (tid < kJoinCols && col < total) {
