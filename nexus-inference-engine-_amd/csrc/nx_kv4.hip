@@ -1,10 +1,14 @@
 // Rows into and out of int4-g32 KV pages.
 //
-// A block takes one page of one kv head, K or V: 16 tokens x hd values, eight
-// to a thread.  Four neighbouring threads hold a group of 32 and agree on its
-// scale through DPP.  Both directions are bound by memory (4.5625 bytes a
-// value); K codes leave the threads as the dwords of their page, V codes, whose
-// dwords hold four tokens each, cross through LDS.
+// A block takes one page of one kv head, K and V: 16 tokens x hd values of
+// each, eight of each to a thread.  Four neighbouring threads hold a group of
+// 32 and agree on its scale through DPP.  Both directions are bound by memory
+// (4.5625 bytes a value), so everything a block reads is requested together:
+// the rows with the table entry, which they do not depend on, K's with V's.  K
+// codes leave the threads as the dwords of their page, V codes, whose dwords
+// hold four tokens each, cross through LDS.  8192 tokens of 8 kv heads of 128
+// (76 MB): 13.8 us in, 16.3 us out, 40 us by turns, when each waits for the
+// other's rows to leave the caches.
 #include "nx_kvc.h"
 
 namespace nx {
@@ -17,15 +21,13 @@ __device__ inline uint32_t dpp_u(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
 }
 
-// The page a block works on (row_page), and its record of head h: null where
-// no row lies in it, the positions are refused or the table names no block of
-// the pool.
+// Offset of a page's record of head h in its pool: -1 where no row lies in the
+// page, the positions are refused or the table names no block of the pool.
 template <int HD>
-__device__ inline uint8_t* page_record(const RowArgs& a, const RowPage& p, int b, int h, bool v) {
-    if (p.none || p.refused) return nullptr;
+__device__ inline int64_t page_record(const RowArgs& a, const RowPage& p, int b, int h) {
+    if (p.none || p.refused) return -1;
     const int blk = a.table[(size_t)b * a.max_blocks + p.page];
-    if (blk < 0 || blk >= a.num_blocks) return nullptr;
-    return (v ? a.vpool : a.kpool) + ((size_t)blk * a.hkv + h) * page_bytes(HD);
+    return blk < 0 || blk >= a.num_blocks ? -1 : ((int64_t)blk * a.hkv + h) * page_bytes(HD);
 }
 
 // Scale of a group from the largest magnitude's bits over the thread's
@@ -38,51 +40,85 @@ __device__ inline uint16_t group_scale(uint32_t amax) {
     return f2h_bits(fminf(__fdiv_rn(__builtin_bit_cast(float, amax), 7.0f), 65504.0f));
 }
 
-// Code 0..15 of x: the quotient rounded to fp32, then half away from zero.
-__device__ inline uint32_t code_of(float x, float s) {
-    if (!(s > 0.0f)) return 8u;  // scale 0 or NaN
-    const float r = fminf(fmaxf(roundf(__fdiv_rn(x, s)), -8.0f), 7.0f);
-    return (uint32_t)((int)r + 8);
+// code - 8 of x, as a float: the quotient x / s rounded to fp32, then half away
+// from zero, in [-8, 7]; `r` is 1 / s, rounded.  With a rounded reciprocal one
+// step of Markstein's iteration gives the rounded quotient (IBM J. Res. Dev. 34
+// (1), 1990; s has 11 bits, and quotients that underflow are far from a half): 3
+// instructions a value where a division takes ten (one token of 8 sequences: 3.7
+// against 4.0 us).
+__device__ inline float step_of(float x, float s, float r) {
+    const float q0 = x * r, q = __builtin_fmaf(__builtin_fmaf(-q0, s, x), r, q0);
+    const float t = __builtin_truncf(q);
+    const float n = t + (fabsf(q - t) >= 0.5f ? __builtin_copysignf(1.0f, q) : 0.0f);
+    return __builtin_amdgcn_fmed3f(n, -8.0f, 7.0f);
 }
+
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+// A thread's eight values of a row, zeros where it has none.
+struct Eight {
+    f4_t lo, hi;
+    __device__ void load(const float* p) {
+        lo = reinterpret_cast<const f4_t*>(p)[0];
+        hi = reinterpret_cast<const f4_t*>(p)[1];
+    }
+    __device__ float operator[](int j) const { return j < 4 ? lo[j] : hi[j - 4]; }
+    __device__ uint16_t scale() const {
+        uint32_t amax = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = (*this)[j];
+            amax = max(amax, __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu);
+        }
+        return group_scale(amax);
+    }
+    // the values' codes less 8 (zeros for a scale of 0 or NaN)
+    __device__ void steps(uint16_t s16, float (&n)[8]) const {
+        const float s = h2f_bits(s16), r = __fdiv_rn(1.0f, s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) n[j] = s > 0.0f ? step_of((*this)[j], s, r) : 0.0f;
+    }
+};
 
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void k_append_int4(RowArgs a) {
     constexpr int S = HD / 32, C = HD / 8;
-    const int h = blockIdx.y >> 1, b = blockIdx.z, tid = threadIdx.x;
-    const bool v = blockIdx.y & 1;
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const RowPage pr = row_page(a.start[b], a.tokens, a.max_blocks, blockIdx.x);
-    uint8_t* rec = page_record<HD>(a, pr, b, h, v);
-    if (!rec) return;
+    if (pr.none || pr.refused) return;
     const int t = tid / C, c = tid % C, row = pr.row0 + t;
     const bool have = row >= 0 && row < a.tokens;
-    float x[8] = {};
+    Eight xk{}, xv{};
     if (have) {
-        const float4* src = reinterpret_cast<const float4*>((v ? a.v : a.k) + (((size_t)b * a.tokens + row) * a.hkv + h) * HD + 8 * c);
-        const float4 lo = src[0], hi = src[1];
-        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+        const size_t at = (((size_t)b * a.tokens + row) * a.hkv + h) * HD + 8 * c;
+        xk.load(a.k + at);
+        xv.load(a.v + at);
     }
-    uint32_t amax = 0u;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max(amax, __builtin_bit_cast(uint32_t, x[j]) & 0x7FFFFFFFu);
-    const uint16_t s16 = group_scale(amax);
-    const float s = h2f_bits(s16);
-    uint16_t* scales = reinterpret_cast<uint16_t*>(rec + 8 * HD);
-    if (have && c % 4 == 0) scales[scale_at(HD, t, c / 4)] = s16;
-    uint32_t* words = reinterpret_cast<uint32_t*>(rec);
-    if (!v) {
-        uint32_t w = 0u;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w |= code_of(x[j], s) << (4 * k_nib(j));
-        if (have) words[k_word(HD, t, 8 * c)] = w;
-        return;
-    }
+    const int64_t rec = page_record<HD>(a, pr, b, h);
+    if (rec < 0) return;
+    const uint16_t sk = xk.scale(), sv = xv.scale();
     __shared__ uint8_t codes[kPage * HD];
-    uint32_t w[2] = {0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j / 4] |= code_of(x[j], s) << (8 * (j % 4));
-    *reinterpret_cast<uint2*>(codes + t * HD + 8 * c) = make_uint2(w[0], w[1]);
+    // codes are gathered as digits of exact floats: four of 4 bits for K (even
+    // j in the low half of the dword, odd j in the high), two of 8 for V
+    float q[8];
+    xk.steps(sk, q);
+    auto digits = [](float a, float b, float c, float d) {
+        return (uint32_t)__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(d, 16.0f, c), 16.0f, b), 16.0f, a + (float)0x8888);
+    };
+    const uint32_t w = digits(q[0], q[2], q[4], q[6]) | digits(q[1], q[3], q[5], q[7]) << 16;
+    xv.steps(sv, q);
+    auto bytes = [](float a, float b) { return (uint32_t)__builtin_fmaf(b, 256.0f, a + (float)0x0808); };
+    const uint32_t w2[2] = {bytes(q[0], q[1]) | bytes(q[2], q[3]) << 16, bytes(q[4], q[5]) | bytes(q[6], q[7]) << 16};
+    if (have) {
+        reinterpret_cast<uint32_t*>(a.kpool + rec)[k_word(HD, t, 8 * c)] = w;
+        if (c % 4 == 0) {
+            reinterpret_cast<uint16_t*>(a.kpool + rec + 8 * HD)[scale_at(HD, t, c / 4)] = sk;
+            reinterpret_cast<uint16_t*>(a.vpool + rec + 8 * HD)[scale_at(HD, t, c / 4)] = sv;
+        }
+    }
+    *reinterpret_cast<uint2*>(codes + t * HD + 8 * c) = make_uint2(w2[0], w2[1]);
     __syncthreads();
-    // thread tid owns dword tid: tokens 4 g + j of dimensions d and d + 16
+    // thread tid owns dword tid of V: tokens 4 g + j of dimensions d and d + 16
     const int i = tid % S, n = (tid / S) % 16, g = tid / S / 16, d = 32 * i + n;
     uint32_t out = 0u, mask = 0u;
 #pragma unroll
@@ -97,6 +133,7 @@ __global__ __launch_bounds__(2 * HD) void k_append_int4(RowArgs a) {
         }
     }
     // tokens of the dword that are not this call's keep their codes
+    uint32_t* words = reinterpret_cast<uint32_t*>(a.vpool + rec);
     if (mask == 0xFFFFFFFFu)
         words[tid] = out;
     else if (mask)
@@ -106,49 +143,46 @@ __global__ __launch_bounds__(2 * HD) void k_append_int4(RowArgs a) {
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void k_read_int4(RowArgs a) {
     constexpr int S = HD / 32, C = HD / 8;
-    const int h = blockIdx.y >> 1, b = blockIdx.z, tid = threadIdx.x;
-    const bool v = blockIdx.y & 1;
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const RowPage pr = row_page(a.start[b], a.tokens, a.max_blocks, blockIdx.x);
     if (pr.none) return;
-    const uint8_t* rec = page_record<HD>(a, pr, b, h, v);
     const int t = tid / C, c = tid % C, row = pr.row0 + t;
     const bool have = row >= 0 && row < a.tokens;
-    float* dst = (v ? a.v : a.k) + (((size_t)b * a.tokens + row) * a.hkv + h) * HD + 8 * c;
-    if (!rec) {
+    const size_t at = have ? (((size_t)b * a.tokens + row) * a.hkv + h) * HD + 8 * c : 0;
+    const int64_t rec = page_record<HD>(a, pr, b, h);
+    if (rec < 0) {
         const float nan = __builtin_nanf("");
-        if (have) {
-            reinterpret_cast<float4*>(dst)[0] = make_float4(nan, nan, nan, nan);
-            reinterpret_cast<float4*>(dst)[1] = make_float4(nan, nan, nan, nan);
-        }
+        if (have)
+            for (float* p : {a.k + at, a.v + at})
+                for (int j = 0; j < 2; ++j) reinterpret_cast<f4_t*>(p)[j] = f4_t{nan, nan, nan, nan};
         return;
     }
-    const float s = h2f_bits(reinterpret_cast<const uint16_t*>(rec + 8 * HD)[scale_at(HD, t, c / 4)]);
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(rec);
-    float x[8];
-    if (!v) {
-        const uint32_t w = words[k_word(HD, t, 8 * c)];
+    const int sat = scale_at(HD, t, c / 4);
+    const uint16_t s16[2] = {reinterpret_cast<const uint16_t*>(a.kpool + rec + 8 * HD)[sat], reinterpret_cast<const uint16_t*>(a.vpool + rec + 8 * HD)[sat]};
+    const uint32_t wk = reinterpret_cast<const uint32_t*>(a.kpool + rec)[k_word(HD, t, 8 * c)], wv = reinterpret_cast<const uint32_t*>(a.vpool + rec)[tid];
+    __shared__ uint8_t codes[kPage * HD];
+    const int i = tid % S, n = (tid / S) % 16, g = tid / S / 16, d = 32 * i + n;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)((int)((w >> (4 * k_nib(j))) & 15u) - 8) * s;
-    } else {
-        __shared__ uint8_t codes[kPage * HD];
-        const uint32_t w = words[tid];
-        const int i = tid % S, n = (tid / S) % 16, g = tid / S / 16, d = 32 * i + n;
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int e = 0; e < 2; ++e) codes[(4 * g + j) * HD + d + 16 * e] = (uint8_t)((wv >> (4 * v_nib(j, 16 * e))) & 15u);
+    __syncthreads();
+    if (!have) return;
+    const uint2 q = *reinterpret_cast<const uint2*>(codes + t * HD + 8 * c);
+    f4_t k[2], v[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) codes[(4 * g + j) * HD + d + 16 * e] = (uint8_t)((w >> (4 * v_nib(j, 16 * e))) & 15u);
-        __syncthreads();
-        const uint2 q = *reinterpret_cast<const uint2*>(codes + t * HD + 8 * c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)((int)(((j < 4 ? q.x : q.y) >> (8 * (j % 4))) & 255u) - 8) * s;
+    for (int j = 0; j < 8; ++j) {
+        k[j / 4][j % 4] = (float)((int)((wk >> (4 * k_nib(j))) & 15u) - 8) * h2f_bits(s16[0]);
+        v[j / 4][j % 4] = (float)((int)(((j < 4 ? q.x : q.y) >> (8 * (j % 4))) & 255u) - 8) * h2f_bits(s16[1]);
     }
-    if (have) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        reinterpret_cast<f4_t*>(a.k + at)[j] = k[j];
+        reinterpret_cast<f4_t*>(a.v + at)[j] = v[j];
     }
 }
 
-dim3 row_grid(const RowArgs& a) { return dim3((unsigned)row_pages(a.tokens), (unsigned)(2 * a.hkv), (unsigned)a.batch); }
+dim3 row_grid(const RowArgs& a) { return dim3((unsigned)row_pages(a.tokens), (unsigned)a.hkv, (unsigned)a.batch); }
 
 }  // namespace
 
