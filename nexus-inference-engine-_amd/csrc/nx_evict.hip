@@ -323,52 +323,45 @@ __device__ inline size_t lane64(size_t v, int l) {
 
 // Tokens into one page of one kv head.  Lane t < 16 has the record (byte
 // offset `src`) and the slot there (`u`) of the token that slot t takes, `moved`
-// has a bit for each t that takes one.  All of a step's loads are requested
+// has a bit for each t that takes one.  All of a wavefront's loads are requested
 // before its stores; a lane alone writes the words it reads.
+// fp16 pages: part 0 is K, part 1 + i the 64 dimensions from 64 i on of V.
 template <int HD>
-__device__ inline void move_f16(const EvictArgs& a, size_t dst, size_t src, int u, unsigned moved, int lane) {
-    // K: 16 bytes of a vector a lane
-    constexpr int KL = HD / 8, KT = kWave / KL < kPage ? kWave / KL : kPage, KN = kPage / KT;  // lanes of a vector, vectors and steps
-    u4_t k[KN] = {};
+__device__ inline void move_f16(const EvictArgs& a, int part, size_t dst, size_t src, int u, unsigned moved, int lane) {
+    if (part == 0) {  // 16 bytes of a vector a lane
+        constexpr int KL = HD / 8, KT = kWave / KL < kPage ? kWave / KL : kPage, KN = kPage / KT;  // lanes of a vector, vectors and steps
+        u4_t k[KN] = {};
 #pragma unroll
-    for (int i = 0; i < KN; ++i) {
-        const int t = i * KT + lane / KL;
-        const size_t p = __shfl(src, t, kWave) + 2 * HD * __shfl(u, t, kWave);
-        if (moved >> t & 1u) k[i] = reinterpret_cast<const u4_t*>(a.kpool + p)[lane % KL];
-    }
-    // V: a dimension's 16 tokens a lane, as one row
-    constexpr int VN = HD / kWave;
-    uint16_t v[kPage][VN] = {};
-    u4_t row[VN][2];
-#pragma unroll
-    for (int i = 0; i < VN; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) row[i][j] = reinterpret_cast<const u4_t*>(a.vpool + dst)[2 * (i * kWave + lane) + j];
-#pragma unroll
-    for (int t = 0; t < kPage; ++t)
-        if (moved >> t & 1u) {
-            const uint16_t* from = reinterpret_cast<const uint16_t*>(a.vpool + lane64(src, t)) + __builtin_amdgcn_readlane(u, t);
-#pragma unroll
-            for (int i = 0; i < VN; ++i) v[t][i] = from[(i * kWave + lane) * kPage];
+        for (int i = 0; i < KN; ++i) {
+            const int t = i * KT + lane / KL;
+            const size_t p = __shfl(src, t, kWave) + 2 * HD * __shfl(u, t, kWave);
+            if (moved >> t & 1u) k[i] = reinterpret_cast<const u4_t*>(a.kpool + p)[lane % KL];
         }
 #pragma unroll
-    for (int i = 0; i < KN; ++i) {
-        const int t = i * KT + lane / KL;
-        if (moved >> t & 1u) reinterpret_cast<u4_t*>(a.kpool + dst + 2 * HD * t)[lane % KL] = k[i];
+        for (int i = 0; i < KN; ++i) {
+            const int t = i * KT + lane / KL;
+            if (moved >> t & 1u) reinterpret_cast<u4_t*>(a.kpool + dst + 2 * HD * t)[lane % KL] = k[i];
+        }
+        return;
     }
+    // a dimension's 16 tokens a lane, written as one row
+    const int d = (part - 1) * kWave + lane;
+    uint16_t v[kPage] = {};
+    u4_t row[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) row[j] = reinterpret_cast<const u4_t*>(a.vpool + dst)[2 * d + j];
 #pragma unroll
     for (int t = 0; t < kPage; ++t)
         if (moved >> t & 1u)
+            v[t] = (reinterpret_cast<const uint16_t*>(a.vpool + lane64(src, t)) + __builtin_amdgcn_readlane(u, t))[(uint32_t)d * kPage];
 #pragma unroll
-            for (int i = 0; i < VN; ++i) {
-                uint32_t w = row[i][t / 8][t / 2 % 4];
-                w = t % 2 ? (w & 0xFFFFu) | (uint32_t)v[t][i] << 16 : (w & 0xFFFF0000u) | v[t][i];
-                row[i][t / 8][t / 2 % 4] = w;
-            }
+    for (int t = 0; t < kPage; ++t)
+        if (moved >> t & 1u) {
+            const uint32_t w = row[t / 8][t / 2 % 4];
+            row[t / 8][t / 2 % 4] = t % 2 ? (w & 0xFFFFu) | (uint32_t)v[t] << 16 : (w & 0xFFFF0000u) | v[t];
+        }
 #pragma unroll
-    for (int i = 0; i < VN; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) reinterpret_cast<u4_t*>(a.vpool + dst)[2 * (i * kWave + lane) + j] = row[i][j];
+    for (int j = 0; j < 2; ++j) reinterpret_cast<u4_t*>(a.vpool + dst)[2 * d + j] = row[j];
 }
 
 template <int HD>
@@ -436,10 +429,13 @@ __device__ inline void move_int4(const EvictArgs& a, size_t dst, size_t src, int
         for (int i = 0; i < S; ++i) own[i] = d[i];
 }
 
-// The first blocks of a (kv head, sequence) take kMoveWaves pages of kept slots
-// each, the others clear kClearSlots slots' weights and tags beyond them.  The
+// The first blocks of a (kv head, sequence) take the pages of kept slots,
+// kParts wavefronts to a page, the others clear kClearSlots slots' weights and tags beyond them.  The
 // weights' outputs may be their inputs: a slot that a token leaves is cleared
 // by the lane that has read it, every other by its own.
+template <int HD, bool INT4>
+constexpr int kParts = INT4 ? 1 : 1 + HD / kWave;  // wavefronts of a page
+
 template <int HD, bool INT4>
 __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
     constexpr int BYTES = INT4 ? page_bytes(HD) : 2 * kPage * HD;
@@ -447,7 +443,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
     const Seq seq = *seq_of(a, b);
     if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.lens_out[b] = seq.len;
     if (seq.len < 0) return;
-    const int cap = a.max_blocks * kPage, ks = kept_slots(a.max_blocks, a.keep), blocks = (ks / kPage + kMoveWaves - 1) / kMoveWaves;
+    const int cap = a.max_blocks * kPage, ks = kept_slots(a.max_blocks, a.keep), blocks = (ks / kPage * kParts<HD, INT4> + kMoveWaves - 1) / kMoveWaves;
     const size_t at = ((size_t)b * a.hkv + h) * cap;
     const Row r = row_of(a, b, h);
     const int tokens = seq.cut ? a.seen[b] - seq.ahead + 1 : seq.len;  // cached before
@@ -460,7 +456,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
         }
         return;
     }
-    const int page = blockIdx.x * kMoveWaves + wave;
+    const int unit = blockIdx.x * kMoveWaves + wave, page = unit / kParts<HD, INT4>, part = unit % kParts<HD, INT4>;
     if (page * kPage >= ks) return;
     // lane t < 16: slot t of the page
     const int s = page * kPage + (lane & 15), bit = s % kWave;
@@ -474,8 +470,8 @@ __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
     const bool takes = used && !(stays >> bit & 1ull);
     int from = 0, tag = 0;
     float w = 0.0f;
-    if (used) {
-        from = takes ? r.from[free_before + __popcll(~stays & ((1ull << bit) - 1ull))] : s;
+    if (used) from = takes ? r.from[free_before + __popcll(~stays & ((1ull << bit) - 1ull))] : s;
+    if (used && part == 0) {
         const int t = a.tags_in[at + from];
         tag = t > 0 ? t : seq.ahead + from;
         w = a.weights_in[at + from];
@@ -488,8 +484,9 @@ __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
         if constexpr (INT4)
             move_int4<HD>(a, dst, src, from % kPage, moved, lane);
         else
-            move_f16<HD>(a, dst, src, from % kPage, moved, lane);
+            move_f16<HD>(a, part, dst, src, from % kPage, moved, lane);
     }
+    if (part > 0) return;
     if (lane < kPage && (used || s >= tokens || !(stays >> bit & 1ull))) {
         a.weights_out[at + s] = w;
         a.tags_out[at + s] = tag;
@@ -503,7 +500,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
 template <int HD, bool INT4>
 void move_case(const EvictArgs& a, hipStream_t st) {
     const int ks = kept_slots(a.max_blocks, a.keep), rest = a.max_blocks * kPage - ks;
-    const unsigned blocks = (unsigned)((ks / kPage + kMoveWaves - 1) / kMoveWaves + (rest + kClearSlots - 1) / kClearSlots);
+    const unsigned blocks = (unsigned)((ks / kPage * kParts<HD, INT4> + kMoveWaves - 1) / kMoveWaves + (rest + kClearSlots - 1) / kClearSlots);
     hipLaunchKernelGGL((k_move<HD, INT4>), dim3(blocks, (unsigned)a.hkv, (unsigned)a.batch), dim3(kMoveThreads), 0, st, a);
 }
 
