@@ -653,12 +653,20 @@ AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4
     p.groups = (G + kHeadsPerBlock - 1) / kHeadsPerBlock;
     p.heads = std::min(G, kHeadsPerBlock);
     p.rec = (p.heads * (hd + 2) + 3) / 4 * 4;
-    // as many blocks as the device holds at once (a second round of them would
-    // begin when the first is done: 27.5 against 26 us for 8 fp16 sequences of
-    // 4K), and a pair of pages at least to a wavefront
+    // Blocks run in rounds of as many as the device holds at once; a round
+    // takes the time of a wavefront's pairs and, before and after them, of about
+    // two more (8 fp16 sequences of 4K: 26 us in one round of 256 blocks, 27.5 in
+    // two).  Fewer splits among equals: fewer records.
     const int64_t rows = (int64_t)batch * hkv * p.groups;
     const int64_t room = (int64_t)device_cus() * (int4 ? weights ? held<true, true>(hd) : held<true, false>(hd) : held<false, true>(hd));
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({room / rows, (pairs + kWaves - 1) / kWaves, kMaxSplits}));
+    int64_t least = INT64_MAX;
+    for (int s = 1; s <= kMaxSplits && (s == 1 || s <= (pairs + kWaves - 1) / kWaves); ++s) {
+        const int64_t cost = ((rows * s + room - 1) / room) * ((pairs + s * kWaves - 1) / (s * kWaves) + 2);
+        if (cost < least) {
+            least = cost;
+            p.splits = s;
+        }
+    }
     p.join = weights || p.splits > 1;
     return p;
 }
