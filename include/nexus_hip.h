@@ -244,7 +244,8 @@ nx_status nx_attn_decode_paged_tq(nx_ctx* ctx, nx_buf q_f32, nx_buf kc4, nx_buf 
  * reads back as NaN.  Rows of a sequence that would begin below 0 or end
  * beyond max_blocks * 16 are not written, nor are rows whose table entry lies
  * outside [0, num_blocks).  tokens beyond max_blocks * 16: NX_ERR_CAPACITY.
- * Two sequences must not write to one page. */
+ * Two sequences must not write to one page.  hkv up to 4096, batch up to
+ * 65535, max_blocks up to 2^26, as for the calls below. */
 nx_status nx_kv_append_int4(nx_ctx* ctx, nx_buf k_f32, nx_buf v_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
                             nx_buf positions_i32, int batch, int tokens, int hkv, int head_dim, int max_blocks,
                             int num_blocks);
@@ -287,7 +288,8 @@ nx_status nx_attn_decode_paged_f16_acc(nx_ctx* ctx, nx_buf q_f32, nx_buf kpool, 
  * token's slot; pages past it are free.  Each of the three may be its input.  A
  * sequence of at most `keep` tokens moves nothing.  One whose length is out of
  * range or above seen[b], or whose table names a block outside the pool, gets
- * lens_out[b] = -1 and stays as it is.  Sequences must not share pages. */
+ * lens_out[b] = -1 and stays as it is.  No page may belong to two sequences, or
+ * twice to one. */
 nx_status nx_kv_evict_f16(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block_table, nx_buf ctx_lens_i32, nx_buf seen_i32,
                           nx_buf weights_f32, nx_buf tags_i32, nx_buf lens_out_i32, nx_buf weights_out_f32,
                           nx_buf tags_out_i32, int batch, int hkv, int head_dim, int max_blocks, int num_blocks, int keep,

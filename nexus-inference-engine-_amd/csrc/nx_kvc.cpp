@@ -28,7 +28,7 @@ struct OnDevice {
 };
 
 // Largest sizes the kernels' grids and 32-bit slot numbers take.
-constexpr int kMaxBatch = 65535, kMaxHkv = 16384, kMaxGroup = 64, kMaxSlotBlocks = 1 << 26;
+constexpr int kMaxBatch = 65535, kMaxHkv = 4096, kMaxGroup = 64, kMaxSlotBlocks = 1 << 26;
 
 nx_status cache_shape(nx_ctx* ctx, const char* name, int batch, int hkv, int hd, int max_blocks, int num_blocks) {
     if (batch < 1 || hkv < 1 || hd < 1 || max_blocks < 1 || num_blocks < 1)
@@ -91,7 +91,12 @@ nx_status rows_int4(nx_ctx* ctx, const char* name, bool append, nx_buf k, nx_buf
     NX_NEED(ctx, vpool, pool, "vpool");
     NX_NEED(ctx, bt, (size_t)batch * max_blocks * 4, "block_table");
     NX_NEED(ctx, pos, (size_t)batch * 4, "positions");
-    if (append ? kpool == vpool : k == v) return fail(ctx, NX_ERR_INVALID, "%s: K and V need buffers of their own", name);
+    const nx_buf all[] = {k, v, kpool, vpool, bt, pos}, outs[] = {append ? kpool : k, append ? vpool : v};
+    for (nx_buf o : outs) {
+        int n = 0;
+        for (nx_buf b : all) n += b == o;
+        if (n > 1) return fail(ctx, NX_ERR_INVALID, "%s: an output is another buffer of the call", name);
+    }
     nx::kvc::RowArgs a{};
     a.k = dptr<float>(k);
     a.v = dptr<float>(v);
@@ -126,6 +131,10 @@ nx_status attn_kvc(nx_ctx* ctx, const char* name, bool int4, nx_buf q, nx_buf kp
     NX_NEED(ctx, lens, (size_t)batch * 4, "ctx_lens");
     NX_NEED(ctx, out, (size_t)batch * hq * hd * 2, "out");
     if (weights || !int4) NX_NEED(ctx, weights, (size_t)batch * hkv * max_blocks * nx::kPage * 4, "weights");
+    const nx_buf in[] = {q, kpool, vpool, bt, lens};
+    bool clash = out == weights;
+    for (nx_buf b : in) clash = clash || b == out || (weights && b == weights);
+    if (clash) return fail(ctx, NX_ERR_INVALID, "%s: an output is another buffer of the call", name);
     nx::kvc::AttnArgs a{};
     if (ctx->device < 0) return fail(ctx, NX_ERR_NO_DEVICE, "%s: no device", name);
     const OnDevice on(ctx->device);

@@ -255,7 +255,7 @@ def test_refusals(op):
             assert call(op, ids, dict(SHAPE, **{name: bad}))[0] == 1, name
     for hd in (32, 96, 80, 512):
         assert call(op, ids, dict(SHAPE, hd=hd))[0] == 4
-    for name, big in (("batch", 65536), ("hkv", 16385), ("max_blocks", (1 << 26) + 1), ("max_blocks", (1 << 31) - 1)):
+    for name, big in (("batch", 65536), ("hkv", 4097), ("max_blocks", (1 << 26) + 1), ("max_blocks", (1 << 31) - 1)):
         assert call(op, ids, dict(SHAPE, hq=big * 4 if name == "hkv" else 8, **{name: big}))[0] == 4, name
     # sizes whose product passes 64 bits would wrap: they are larger than any buffer
     assert call(op, ids, dict(SHAPE, num_blocks=(1 << 31) - 1))[0] == 1
@@ -273,6 +273,10 @@ def test_refusals(op):
         assert call(op, ids, dict(SHAPE, hq=0))[0] == 1
         assert call(op, ids, dict(SHAPE, hq=130))[0] == 4
         assert call(op, ids[:6] + [0], SHAPE)[0] == (6 if "int4" in op else 1)
+        for out in (5, 6):  # the output and the weights are buffers of their own
+            for i in range(n):
+                if i != out:
+                    assert call(op, ids[:out] + [ids[i]] + ids[out + 1:], SHAPE, [1 << 20] * n)[0] == 1
     elif "evict" in op:
         for keep, recent in ((0, 0), (-1, 0), (4, 5), (4, -1)):
             assert call(op, ids, dict(SHAPE, keep=keep, recent=recent))[0] == 1
@@ -287,8 +291,10 @@ def test_refusals(op):
     else:
         assert call(op, ids, dict(SHAPE, tokens=0))[0] == 1
         assert call(op, ids, dict(SHAPE, tokens=49))[0] == 7
-        two = [1, 2, 3, 3, 5, 6] if "append" in op else [1, 2, 3, 4, 5, 5]
-        assert call(op, two, SHAPE, [1 << 20] * n)[0] == 1
+        for out in ((2, 3) if "append" in op else (4, 5)):
+            for i in range(n):
+                if i != out:
+                    assert call(op, ids[:out] + [ids[i]] + ids[out + 1:], SHAPE, [1 << 20] * n)[0] == 1
 
 
 # ---------------------------------------------------------- append and read --
