@@ -245,7 +245,7 @@ nx_status nx_attn_decode_paged_tq(nx_ctx* ctx, nx_buf q_f32, nx_buf kc4, nx_buf 
  * beyond max_blocks * 16 are not written, nor are rows whose table entry lies
  * outside [0, num_blocks).  tokens beyond max_blocks * 16: NX_ERR_CAPACITY.
  * Two sequences must not write to one page.  hkv up to 4096, batch up to
- * 65535, max_blocks up to 2^26, as for the calls below. */
+ * 65535, max_blocks up to 2^22, as for the calls below. */
 nx_status nx_kv_append_int4(nx_ctx* ctx, nx_buf k_f32, nx_buf v_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
                             nx_buf positions_i32, int batch, int tokens, int hkv, int head_dim, int max_blocks,
                             int num_blocks);
@@ -263,7 +263,10 @@ nx_status nx_kv_read_int4(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block_
  * slots at ctx_lens[b] and above are left as they are.  A sequence whose
  * length exceeds max_blocks * 16 (or is negative), or whose table names a block
  * outside [0, num_blocks) for one of its pages, gets NaN output rows and its
- * weights stay as they are. */
+ * weights stay as they are.  A cached value of its positions that is not
+ * finite makes outputs NaN or infinite (K: its kv head's, and the weights; V:
+ * its dimension's, of int4 pages its group's); slots past the length may hold
+ * anything.  No output or weights buffer may be another buffer of the call. */
 nx_status nx_attn_decode_paged_int4(nx_ctx* ctx, nx_buf q_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
                                     nx_buf ctx_lens_i32, nx_buf out_f16, nx_buf weights_f32, int batch, int hq, int hkv,
                                     int head_dim, int max_blocks, int num_blocks);
@@ -383,7 +386,8 @@ nx_status nx_init_kv_cache(nx_ctx* ctx, int num_layers, int max_seq, int n_kv_he
  * workspace the entry points keep per context -- FFN activations, K-part
  * sums (of the down projection, and of GEMMs over a layer's matrices with up
  * to 2048 rows), sampler rows, attention split records, counters and table
- * checks -- to what calls up to these sizes need, so those calls allocate
+ * checks, the compact cache's records, scores and eviction lists (4 bytes a
+ * query head and position, and more) -- to what calls up to these sizes need, so those calls allocate
  * nothing (and may be captured, where they can be at all).  A size of 0 skips its workspace.  The reference reserves staging bytes; this
  * library takes the shapes the bytes come from. */
 nx_status nx_reserve_workspace(nx_ctx* ctx, int batch, int max_ffn, int vocab, int n_heads, int n_kv_heads,

@@ -520,11 +520,10 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
 // Blocks of a kernel that a compute unit holds at once.
 template <int HD, bool INT4, bool ACC>
 int blocks_per_cu() {
-    static int n = 0;
-    if (n == 0) {
+    static const int n = [] {
         int v = 0;
-        n = hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, k_attn<HD, INT4, ACC>, kThreads, 0) == hipSuccess && v > 0 ? v : 1;
-    }
+        return hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, k_attn<HD, INT4, ACC>, kThreads, 0) == hipSuccess && v > 0 ? v : 1;
+    }();
     return n;
 }
 
@@ -645,14 +644,17 @@ int held(int hd) {
     return hd == 64 ? blocks_per_cu<64, INT4, ACC>() : hd == 128 ? blocks_per_cu<128, INT4, ACC>() : blocks_per_cu<256, INT4, ACC>();
 }
 
+// The part of a plan that the heads decide.
+AttnPlan heads_plan(int hq, int hkv, int hd) {
+    const int G = hq / hkv, heads = std::min(G, kHeadsPerBlock);
+    return {(G + kHeadsPerBlock - 1) / kHeadsPerBlock, heads, 1, (heads * (hd + 2) + 3) / 4 * 4, true};
+}
+
 }  // namespace
 
 AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4, bool weights) {
-    AttnPlan p;
-    const int G = hq / hkv, pairs = (max_blocks + 1) / 2;
-    p.groups = (G + kHeadsPerBlock - 1) / kHeadsPerBlock;
-    p.heads = std::min(G, kHeadsPerBlock);
-    p.rec = (p.heads * (hd + 2) + 3) / 4 * 4;
+    AttnPlan p = heads_plan(hq, hkv, hd);
+    const int pairs = (max_blocks + 1) / 2;
     // Blocks run in rounds of as many as the device holds at once; a round
     // takes the time of a wavefront's pairs and, before and after them, of about
     // two more (8 fp16 sequences of 4K: 26 us in one round of 256 blocks, 27.5 in
@@ -672,6 +674,11 @@ AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4
 }
 
 size_t attn_part_floats(const AttnPlan& p, int batch, int hkv) { return (size_t)batch * hkv * p.groups * p.splits * p.rec; }
+size_t attn_most_part_floats(int batch, int hq, int hkv, int hd) {
+    AttnPlan p = heads_plan(hq, hkv, hd);
+    p.splits = kMaxSplits;
+    return attn_part_floats(p, batch, hkv);
+}
 
 hipError_t attn_launch(const AttnArgs& a, bool int4, hipStream_t st) {
     switch (a.hd) {

@@ -28,7 +28,7 @@ struct OnDevice {
 };
 
 // Largest sizes the kernels' grids and 32-bit slot numbers take.
-constexpr int kMaxBatch = 65535, kMaxHkv = 4096, kMaxGroup = 64, kMaxSlotBlocks = 1 << 26;
+constexpr int kMaxBatch = 65535, kMaxHkv = 4096, kMaxGroup = 64, kMaxSlotBlocks = 1 << 22;
 
 nx_status cache_shape(nx_ctx* ctx, const char* name, int batch, int hkv, int hd, int max_blocks, int num_blocks) {
     if (batch < 1 || hkv < 1 || hd < 1 || max_blocks < 1 || num_blocks < 1)
@@ -217,11 +217,9 @@ namespace nx {
 nx_status kvc_reserve(nx_ctx* ctx, int batch, int hq, int hkv, int hd, int max_ctx) {
     if (hd != 64 && hd != 128 && hd != 256) return NX_OK;
     const int blocks = (max_ctx + kPage - 1) / kPage;
-    size_t bytes = 4 * kvc::evict_ws_words(batch, hkv, blocks, blocks * kPage);
-    // (a smaller batch may split its pages further)
-    for (int b = 1; b <= batch; ++b)
-        for (bool int4 : {false, true})
-            bytes = std::max(bytes, attn_ws_bytes(kvc::attn_plan(b, hq, hkv, hd, blocks, int4, true), b, hq, hkv, blocks, true));
+    // (a call of less may split its pages further: records for the most splits)
+    const size_t attn = 4 * (kvc::attn_most_part_floats(batch, hq, hkv, hd) + kvc::attn_raw_floats(batch, hq, blocks));
+    const size_t bytes = std::max(4 * kvc::evict_ws_words(batch, hkv, blocks, blocks * kPage), attn);
     return kvc_ws(ctx, bytes, "nx_reserve_workspace");
 }
 }  // namespace nx

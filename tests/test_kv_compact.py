@@ -145,7 +145,12 @@ def cache(rng, int4, lens, hkv, hd, max_blocks, nblk, amp=1.0, stale=np.nan):
     """Pools as the library holds them, their values in 64 bits, and the table.
     Tokens past the lengths hold `stale`, table entries past them nonsense."""
     B = len(lens)
-    table = table_of(rng, B, max_blocks, nblk)
+    if nblk >= B * max_blocks:
+        table = table_of(rng, B, max_blocks, nblk)
+    else:  # pages for the tokens alone
+        table, free = np.zeros((B, max_blocks), np.int32), rng.permutation(nblk).astype(np.int32)
+        for b, n in enumerate(lens):
+            table[b, :-(-n // PAGE)], free = np.split(free, [-(-n // PAGE)])
     ks, vs = ([(rng.normal(0, 1, (n, hkv, hd)) * amp).astype(np.float32) for n in lens] for _ in range(2))
     pk, pv = to_pages(ks, table, nblk, stale), to_pages(vs, table, nblk, stale)
     if int4:
@@ -173,7 +178,7 @@ def test_every_code_has_a_nibble_of_its_own(hd, value):
     assert np.array_equal(unpack(pack(q, s, value), hd, value), want)
 
 
-@pytest.mark.parametrize("max_blocks", [1, 2, 5, 1 << 26])
+@pytest.mark.parametrize("max_blocks", [1, 2, 5, 1 << 22])
 def test_row_pages_stay_inside_the_table(max_blocks):
     """The pages of an append: inside the table, every row in exactly one,
     no more than the launch has; out of range: refused."""
@@ -255,7 +260,7 @@ def test_refusals(op):
             assert call(op, ids, dict(SHAPE, **{name: bad}))[0] == 1, name
     for hd in (32, 96, 80, 512):
         assert call(op, ids, dict(SHAPE, hd=hd))[0] == 4
-    for name, big in (("batch", 65536), ("hkv", 4097), ("max_blocks", (1 << 26) + 1), ("max_blocks", (1 << 31) - 1)):
+    for name, big in (("batch", 65536), ("hkv", 4097), ("max_blocks", (1 << 22) + 1), ("max_blocks", (1 << 31) - 1)):
         assert call(op, ids, dict(SHAPE, hq=big * 4 if name == "hkv" else 8, **{name: big}))[0] == 4, name
     # sizes whose product passes 64 bits would wrap: they are larger than any buffer
     assert call(op, ids, dict(SHAPE, num_blocks=(1 << 31) - 1))[0] == 1
@@ -407,10 +412,10 @@ def test_append_and_read_out_of_range(ctx):
 
 
 # ------------------------------------------------------------------ attention --
-def check_attention(ctx, int4, hq, hkv, hd, lens, weights=True, amp=1.0, spare=2, qamp=1.0, twice=False, seed=0):
+def check_attention(ctx, int4, hq, hkv, hd, lens, weights=True, amp=1.0, spare=2, qamp=1.0, twice=False, seed=0, nblk=0):
     rng = np.random.default_rng(seed + hq * 7 + hd + sum(lens))
     B, mb = len(lens), max(1, -(-max(lens) // PAGE)) + spare
-    nblk = B * mb + 1
+    nblk = nblk or B * mb + 1
     kp, vp, k64, v64, table = cache(rng, int4, lens, hkv, hd, mb, nblk, amp)
     q = (rng.normal(0, 1, (B, hq, hd)) * qamp).astype(np.float32)
     w0 = rng.exponential(1, (B, hkv, mb * PAGE)).astype(np.float32)
@@ -451,6 +456,20 @@ def test_attention(ctx, int4, hq, hkv, hd, lens):
 @pytest.mark.parametrize("hq,hkv,hd,lens", [(4, 2, 64, [0, 40]), (32, 8, 128, [300]), (12, 1, 256, [999, 16])])
 def test_attention_int4_without_weights(ctx, hq, hkv, hd, lens):
     check_attention(ctx, True, hq, hkv, hd, lens, weights=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int4,weights", [(True, True), (True, False), (False, True)], ids=["int4", "int4-plain", "f16"])
+def test_attention_of_many_rows(ctx, int4, weights):
+    """More rows than the device holds blocks, so one block to a row, and one
+    long sequence among short ones: a wavefront's pages pass 64 of the table."""
+    check_attention(ctx, int4, 256, 4, 64, [9001] + [1, 17, 0, 40] * 47, weights=weights, nblk=1100)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int4", [True, False], ids=["int4", "f16"])
+def test_attention_past_the_joins_first_slots(ctx, int4):
+    check_attention(ctx, int4, 9, 1, 64, [40000, 32769])
 
 
 @pytest.mark.gpu
@@ -566,7 +585,9 @@ def run_evict(ctx, int4, h, B, hkv, hd, mb, nblk, keep, recent, alias):
 @pytest.mark.parametrize("hd,hkv,lens,keep,recent,alias", [
     (64, 1, [2], 1, 0, False), (64, 2, [1, 17, 16, 0, 40], 16, 3, True), (128, 2, [100, 33], 37, 37, False),
     (128, 8, [257], 256, 64, True), (256, 1, [300, 64], 63, 0, False), (64, 3, [1500], 700, 100, True),
-    (128, 1, [5000, 4000], 4001, 9, False), (64, 1, [20, 48], 48, 5, False), (64, 1, [20, 48], 1000, 900, True)])
+    (128, 1, [5000, 4000], 4001, 9, False), (64, 1, [20, 48], 48, 5, False), (64, 1, [20, 48], 1000, 900, True),
+    (64, 1, [20000], 3000, 100, False), (64, 1, [40000], 9000, 500, False), (64, 1, [70000, 33000], 30000, 1000, True),
+    (64, 1, [70000], 69990, 69000, False)])
 def test_eviction(ctx, int4, hd, hkv, lens, keep, recent, alias):
     """Tokens, weights, tags and lengths as the plain form has them, twice in a
     row with tokens appended between; no other byte of the pools changes."""
