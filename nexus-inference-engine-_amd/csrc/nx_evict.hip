@@ -213,9 +213,15 @@ __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
         uint32_t base = max(prefix, 1u), span = prefix + (1u << 21) - base;
         const bool few = all <= kListed;
         if (few)
-            over(s0, mine_n, [&](int, uint32_t key) {
-                if (key - base < span) list[atomicAdd(&listed, 1)] = key;
-            });
+            for (int u0 = 0; u0 < mine_n; u0 += 32) {
+                uint32_t hits = 0u;
+                over(s0 + u0 * kWave, min(mine_n - u0, 32), [&](int u, uint32_t key) { hits |= (uint32_t)(key - base < span) << u; });
+                const int n = __popc(hits), upto = wave_scan(n);
+                int at = 0;
+                if (lane == kWave - 1) at = atomicAdd(&listed, upto);
+                at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - n;
+                for (; hits; hits &= hits - 1u) list[at++] = keys[s0 + (u0 + __ffs(hits) - 1) * kWave + lane];
+            }
         for (int shift = 10; shift >= 0; shift -= 10) {
             const uint32_t last = shift ? 2047u : 1023u;
             for (int i = tid; i < kBins; i += kPickThreads) hist[i] = make_uint2(0u, 0u);
