@@ -446,14 +446,13 @@ template <int HD, bool INT4>
 __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
     constexpr int BYTES = INT4 ? page_bytes(HD) : 2 * kPage * HD;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z;
-    const Seq seq = *seq_of(a, b);
-    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.lens_out[b] = seq.len;
-    if (seq.len < 0) return;
     const int cap = a.max_blocks * kPage, ks = kept_slots(a.max_blocks, a.keep), blocks = (ks / kPage * kParts<HD, INT4> + kMoveWaves - 1) / kMoveWaves;
     const size_t at = ((size_t)b * a.hkv + h) * cap;
     const Row r = row_of(a, b, h);
-    const int tokens = seq.cut ? a.seen[b] - seq.ahead + 1 : seq.len;  // cached before
     if ((int)blockIdx.x >= blocks) {
+        const Seq seq = *seq_of(a, b);
+        if (seq.len < 0) return;
+        const int tokens = seq.cut ? a.seen[b] - seq.ahead + 1 : seq.len;  // cached before
         const int first = ks + ((int)blockIdx.x - blocks) * kClearSlots, end = min(cap, first + kClearSlots);
         for (int s = first + (int)threadIdx.x; s < end; s += kMoveThreads) {
             if (s < tokens && (r.stays[s / kWave] >> (s % kWave) & 1ull)) continue;
@@ -464,15 +463,26 @@ __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
     }
     const int unit = blockIdx.x * kMoveWaves + wave, page = unit / kParts<HD, INT4>, part = unit % kParts<HD, INT4>;
     if (page * kPage >= ks) return;
+    // A wavefront's time is the chain from here to the tokens' bytes: what does
+    // not depend on the sequence's state is requested with it (stays and
+    // free_before hold anything where nothing is cut, the table's entry
+    // where the sequence is refused or too short).
+    const int32_t* table = a.table + (size_t)b * a.max_blocks;
+    const Seq seq = *seq_of(a, b);
+    const int seen = a.seen[b], here = table[page];
+    unsigned long long stays = r.stays[page * kPage / kWave];
+    int free_before = r.free_before[page * kPage / kWave];
+    asm volatile("" : "+v"(stays), "+v"(free_before) : "v"(seen), "v"(here));
+    if (unit == 0 && h == 0 && lane == 0) a.lens_out[b] = seq.len;
+    if (seq.len < 0) return;
+    const int tokens = seq.cut ? seen - seq.ahead + 1 : seq.len;
+    if (!seq.cut) {
+        stays = ~0ull;
+        free_before = 0;
+    }
     // lane t < 16: slot t of the page
     const int s = page * kPage + (lane & 15), bit = s % kWave;
     const bool used = s < seq.len && lane < kPage;
-    unsigned long long stays = ~0ull;
-    int free_before = 0;
-    if (seq.cut) {
-        stays = r.stays[page * kPage / kWave];
-        free_before = r.free_before[page * kPage / kWave];
-    }
     const bool takes = used && !(stays >> bit & 1ull);
     int from = 0, tag = 0;
     float w = 0.0f;
@@ -484,9 +494,8 @@ __global__ __launch_bounds__(kMoveThreads) void k_move(EvictArgs a) {
     }
     const unsigned moved = (unsigned)__ballot(takes);
     if (moved) {
-        const int32_t* table = a.table + (size_t)b * a.max_blocks;
         const size_t src = takes ? ((size_t)table[from / kPage] * a.hkv + h) * BYTES : 0;
-        const size_t dst = ((size_t)table[page] * a.hkv + h) * BYTES;
+        const size_t dst = ((size_t)here * a.hkv + h) * BYTES;
         if constexpr (INT4)
             move_int4<HD>(a, dst, src, from % kPage, moved, lane);
         else
