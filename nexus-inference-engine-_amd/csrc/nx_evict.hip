@@ -8,8 +8,9 @@
 // destinations below, and no copy can overtake another.
 //
 // k_pick, one block per (sequence, kv head): a radix selection over 32-bit
-// keys (11, 11 and 10 bits), which stay in LDS, finds the keep-th largest; ballots number the equal ones, the free slots and the
-// tokens that move in slot order.  k_move, one wavefront per destination page:
+// keys (11, 11 and 10 bits), which stay in LDS, finds the keep-th largest;
+// ballots number the equal ones, the free slots and the tokens that move in
+// slot order.  k_move, one wavefront per destination page:
 // weights and tags; K vectors as they are; V, whose pages are dimension-major,
 // by rewriting the page's words, each of which one lane owns.
 #include <algorithm>
@@ -22,7 +23,7 @@ namespace kvc {
 namespace {
 
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / kWave;
-constexpr int kBins = 2048, kListed = 2048;
+constexpr int kBins = 2048, kListed = 2048, kRanked = 128;
 constexpr int kKeyPad = 8 * kWave;  // keys past a row's that a wavefront may read
 constexpr int kLdsSlots = 32768;  // slots whose keys a block holds in LDS
 
@@ -65,9 +66,8 @@ __device__ inline Row row_of(const EvictArgs& a, int b, int h) {
 // Order of weights as unsigned numbers: NaN below every other, -0 as 0; no
 // weight has key 0, which stands for no token.
 __device__ inline uint32_t weight_key(float w) {
-    if (w != w) return 1u;
     const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    return w != w ? 1u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
 // base + the bits of v below this lane.
@@ -104,35 +104,44 @@ __device__ inline int2 block_scan(int2 v, int2* lds, int2& total) {
 }
 
 // SLOTS: the longest row whose keys stay in LDS; 0: they go through memory.
-// A block is one compute unit's work and bound by its instructions and, in the
-// first loop, by what one compute unit can request; a row's slots are passed
-// three times: keys and their top bits are counted, the keys of the bin that
-// holds the keep-th are listed, and the keys are compared with the keep-th.
-// 32768 slots of 8 kv heads: 22 us, 4352: 9 us.
+// A block is one compute unit's work: the first loop is bound by what one
+// compute unit can request and count (32768 slots: 11000 of 37000 cycles), the
+// others by its instructions.  A row's slots are passed three times: keys and
+// their top bits are counted, the keys of the bin that holds the keep-th are
+// listed, and the keys are compared with the keep-th (twice more where some of
+// its equals stay and some go).  8 kv heads of 32768 slots: 17.5 us, of 4352: 8.3 us.
 template <int SLOTS>
 __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
     // two counters per bin, by lane: weights crowd into few bins
     __shared__ uint2 hist[kBins];
     __shared__ uint32_t lds_keys[SLOTS > 0 ? SLOTS + kKeyPad : 1], list[kListed];
     __shared__ int2 sums[kPickWaves];
-    __shared__ int found_bin, found_left, found_all, listed;
+    __shared__ int found, found_left, found_all, listed;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cap = a.max_blocks * kPage, keep = a.keep, L = a.lens_in[b], N = a.seen[b];
     const Row r = row_of(a, b, h);
     const size_t at = ((size_t)b * a.hkv + h) * cap;
     const float* w_in = a.weights_in + at;
     const int32_t* t_in = a.tags_in + at;
+    // the table's entries are requested here and looked at behind the first loop
+    const int32_t* table = a.table + (size_t)b * a.max_blocks;
+    const int entry[2] = {table[min(tid, a.max_blocks - 1)], table[min(tid + kPickThreads, a.max_blocks - 1)]};
+    bool bad = L < 0 || L > cap || N < L;
+    const int pages = bad ? 0 : (L + kPage - 1) / kPage, ahead = (int)((unsigned)N - (unsigned)L + 1u);
+    auto outside = [&] {
+        auto out = [&](int e) { return e < 0 || e >= a.num_blocks; };
+        bool any = (tid < pages && out(entry[0])) || (tid + kPickThreads < pages && out(entry[1]));
+        for (int p = tid + 2 * kPickThreads; p < pages; p += kPickThreads) any = any || out(table[p]);
+        return any;
+    };
+    if (bad || L <= keep) {
+        bad = __syncthreads_or(bad || outside());
+        if (tid == 0 && h == 0) *seq_of(a, b) = {bad ? -1 : L, 0, ahead};
+        return;
+    }
     for (int i = tid; i < kBins; i += kPickThreads) hist[i] = make_uint2(0u, 0u);
     if (tid == 0) listed = 0;
-    bool bad = L < 0 || L > cap || N < L;
-    if (!bad)
-        for (int p = tid; p < (L + kPage - 1) / kPage; p += kPickThreads) {
-            const int blk = a.table[(size_t)b * a.max_blocks + p];
-            bad = bad || blk < 0 || blk >= a.num_blocks;
-        }
-    bad = __syncthreads_or(bad);
-    if (tid == 0 && h == 0) *seq_of(a, b) = {bad ? -1 : min(L, keep), !bad && L > keep, N - L + 1};
-    if (bad || L <= keep) return;
+    __syncthreads();
     uint32_t* keys;
     if constexpr (SLOTS > 0)
         keys = lds_keys;
@@ -155,73 +164,134 @@ __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
                 if (u0 + j < n) f(u0 + j, k[j]);
         }
     };
-    // ---- the keep-th largest key.  Recent tokens have the largest and are
-    // counted apart.
+    // ---- the keep-th largest key.  Recent tokens have the largest, in a bin of
+    // their own (no weight's key is above an infinity's, 0xFF800000).
     uint32_t* count = reinterpret_cast<uint32_t*>(hist) + (lane & 1);
-    int recents = 0;
-    for (int u0 = 0; u0 < mine_n; u0 += 8) {
-        float w[8];
-        int t[8];
+    auto key_of = [&](int s, float w, int t) {
+        uint32_t key = weight_key(w);
+        asm("" : "+v"(key));  // (or it becomes a branch for each key)
+        return (t > 0 ? t : s + ahead) > N - a.recent ? 0xFFFFFFFFu : key;
+    };
+    auto put = [&](int s, uint32_t key) {
+        keys[s] = key;
+        atomicAdd(count + 2 * (key >> 21), 1u);
+    };
+    // eight steps at a time, the next eight requested ahead; then the last few
+    const int full = max(s1 - s0, 0) / (8 * kWave) * 8;
+    float w[8];
+    int t[8];
+    if (full > 0) {
+        auto request = [&](int u) {
+            const float* wp = w_in + s0 + u * kWave + lane;
+            const int32_t* tp = t_in + s0 + u * kWave + lane;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = wp[j * kWave];
+                t[j] = tp[j * kWave];
+            }
+        };
+        request(0);
+        for (int u0 = 0; u0 < full; u0 += 8) {
+            const int s = s0 + u0 * kWave + lane;
+            uint32_t key[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) key[j] = key_of(s + j * kWave, w[j], t[j]);
+            request(min(u0 + 8, full - 8));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) put(s + j * kWave, key[j]);
+        }
+    }
+    if (full < mine_n) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int s = min(s0 + (u0 + j) * kWave + lane, s1 - 1);
+            const int s = min(s0 + (full + j) * kWave + lane, s1 - 1);
             w[j] = w_in[s];
             t[j] = t_in[s];
         }
+        uint32_t key[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (u0 + j >= mine_n) break;
-            const int s = s0 + (u0 + j) * kWave + lane, tag = t[j] > 0 ? t[j] : N - L + s + 1;
-            const bool in = s < s1, recent = in && tag > N - a.recent;
-            const uint32_t key = recent ? 0xFFFFFFFFu : in ? weight_key(w[j]) : 0u;
-            keys[s] = key;
-            recents += recent;
-            if (key - 1u < 0xFFFFFFFEu) atomicAdd(count + 2 * (key >> 21), 1u);
+            const int s = s0 + (full + j) * kWave + lane;
+            key[j] = s < s1 ? key_of(s, w[j], t[j]) : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int s = s0 + (full + j) * kWave + lane;
+            if (s < s1)
+                put(s, key[j]);
+            else if (full + j < mine_n)
+                keys[s] = 0u;
         }
     }
-    __syncthreads();
+    bad = __syncthreads_or(outside());
+    if (tid == 0 && h == 0) *seq_of(a, b) = {bad ? -1 : keep, !bad, ahead};
+    if (bad) return;
     int2 total;
     uint32_t prefix = 0u;
-    int left = 0, all = 0;
+    int left = keep, all = 0;
     // The bin of the counts in which the left-th largest lies: thread i adds up
     // bins 2047 - 2 i and 2046 - 2 i, the largest keys first.
-    auto find = [&](int shift, bool first_pass) {
+    auto find = [&](int shift) {
         const uint2 x = hist[kBins - 1 - 2 * tid], y = hist[kBins - 2 - 2 * tid];
         const int hi = (int)(x.x + x.y), lo = (int)(y.x + y.y);
-        const int before = block_scan(make_int2(hi + lo, recents), sums, total).x;
-        if (first_pass) left = keep - total.y;
+        const int before = block_scan(make_int2(hi + lo, 0), sums, total).x;
         if (before < left && left <= before + hi + lo) {
             const bool first = left <= before + hi;
-            found_bin = first ? kBins - 1 - 2 * tid : kBins - 2 - 2 * tid;
+            found = first ? kBins - 1 - 2 * tid : kBins - 2 - 2 * tid;
             found_left = left - before - (first ? 0 : hi);
             found_all = first ? hi : lo;
         }
         __syncthreads();
-        if (left <= 0) return;
-        prefix |= (uint32_t)found_bin << shift;
+        prefix |= (uint32_t)found << shift;
         left = found_left;
         all = found_all;
     };
-    find(21, true);
-    if (left <= 0) {
-        prefix = 0xFFFFFFFFu;
-        left = keep;
-        all = total.y;
-    } else {
-        // the bin's keys in a list, if they are few, so that the other bits
-        // take no more passes over the row
-        uint32_t base = max(prefix, 1u), span = prefix + (1u << 21) - base;
-        const bool few = all <= kListed;
-        if (few)
-            for (int u0 = 0; u0 < mine_n; u0 += 32) {
-                uint32_t hits = 0u;
-                over(s0 + u0 * kWave, min(mine_n - u0, 32), [&](int u, uint32_t key) { hits |= (uint32_t)(key - base < span) << u; });
-                const int n = __popc(hits), upto = wave_scan(n);
-                int at = 0;
-                if (lane == kWave - 1) at = atomicAdd(&listed, upto);
-                at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - n;
-                for (; hits; hits &= hits - 1u) list[at++] = keys[s0 + (u0 + __ffs(hits) - 1) * kWave + lane];
+    find(21);
+    // the bin's keys in a list, if they are few, so that the other bits take no
+    // more passes over the row
+    uint32_t base = max(prefix, 1u), span = prefix + (1u << 21) - base;
+    const bool few = all <= kListed;
+    if (few)
+        for (int u0 = 0; u0 < mine_n; u0 += 32) {
+            uint32_t hits = 0u;
+            over(s0 + u0 * kWave, min(mine_n - u0, 32), [&](int u, uint32_t key) { hits |= (uint32_t)(key - base < span) << u; });
+            const int n = __popc(hits), upto = wave_scan(n);
+            int at = 0;
+            if (lane == kWave - 1) at = atomicAdd(&listed, upto);
+            at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - n;
+            for (; hits; hits &= hits - 1u) list[at++] = keys[s0 + (u0 + __ffs(hits) - 1) * kWave + lane];
+        }
+    if (all <= kRanked) {
+        // each key's number of larger ones (<< 16) and of equal ones, wavefront w
+        // against keys w, w + 16, ..: two passes over the other bits take longer
+        // (4352 slots: 4100 against 1500 cycles)
+        uint32_t* rank = reinterpret_cast<uint32_t*>(hist);
+        const int n = all;
+        if (tid < n) rank[tid] = 0u;
+        __syncthreads();
+        for (int i0 = 0; i0 < n; i0 += kWave) {
+            const uint32_t key = list[min(i0 + lane, n - 1)];
+            uint32_t c = 0u;
+            for (int j = wave; j < n; j += kPickWaves) {
+                const uint32_t other = list[j];
+                c += other > key ? 1u << 16 : other == key ? 1u : 0u;
             }
+            if (i0 + lane < n) atomicAdd(rank + i0 + lane, c);
+        }
+        __syncthreads();
+        if (tid < n) {
+            const int larger = (int)(rank[tid] >> 16), same = (int)(rank[tid] & 0xFFFFu);
+            if (larger < left && left <= larger + same) {  // (equal keys all write the same)
+                found = (int)list[tid];
+                found_left = left - larger;
+                found_all = same;
+            }
+        }
+        __syncthreads();
+        prefix = (uint32_t)found;
+        left = found_left;
+        all = found_all;
+    } else {
         for (int shift = 10; shift >= 0; shift -= 10) {
             const uint32_t last = shift ? 2047u : 1023u;
             for (int i = tid; i < kBins; i += kPickThreads) hist[i] = make_uint2(0u, 0u);
@@ -234,7 +304,7 @@ __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
             else
                 over(s0, mine_n, add);
             __syncthreads();
-            find(shift, false);
+            find(shift);
             base = max(prefix, 1u);
             span = prefix + (1u << shift) - base;
             __syncthreads();
@@ -436,9 +506,12 @@ __device__ inline void move_int4(const EvictArgs& a, size_t dst, size_t src, int
 }
 
 // The first blocks of a (kv head, sequence) take the pages of kept slots,
-// kParts wavefronts to a page, the others clear kClearSlots slots' weights and tags beyond them.  The
-// weights' outputs may be their inputs: a slot that a token leaves is cleared
-// by the lane that has read it, every other by its own.
+// kParts wavefronts to a page, the others clear kClearSlots slots' weights and
+// tags beyond them.  The weights' outputs may be their inputs: a slot that a
+// token leaves is cleared by the lane that has read it, every other by its own.
+// fp16: bound by memory, since V's pages are dimension-major, so that a token
+// moves with whole pages: 8 sequences of 8192 tokens of 8 kv heads of 128 cut to
+// 2048 read 169 MB and write 66, 54 us; int4, one of 32768 cut to 4096: 8 us.
 template <int HD, bool INT4>
 constexpr int kParts = INT4 ? 1 : 1 + HD / kWave;  // wavefronts of a page
 
