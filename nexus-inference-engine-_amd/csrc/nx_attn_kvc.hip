@@ -5,7 +5,7 @@
 // kv head for up to 8 of its query heads, keeps an online softmax per head,
 // merges its wavefronts through LDS and writes one record (O, M, L), or the
 // fp16 output where it has the kv head to itself.  With weights it also writes
-// the scores.  k_join: merges the records and, with weights, turns the scores
+// the scores, and with the kv head to itself it adds the weights as well.  k_join: merges the records and, with weights, turns the scores
 // into exp(s - M) / L, whose sum over the query heads of the kv head it adds to
 // the weights.  (The scores need M and L of all splits, which no block of k_attn
 // has; reading them back costs 8 bytes a token and query head, the pages again
@@ -391,6 +391,9 @@ __device__ inline void store_out(uint16_t* out, f4_t v) {
         make_uint2((uint32_t)f2h_bits(v[0]) | ((uint32_t)f2h_bits(v[1]) << 16), (uint32_t)f2h_bits(v[2]) | ((uint32_t)f2h_bits(v[3]) << 16));
 }
 
+// The weight of a score, from its head's M and 1 / L.
+__device__ inline float part_of(float score, float2 norm) { return __builtin_amdgcn_exp2f(score - norm.x) * norm.y; }
+
 template <int HD, bool INT4, bool ACC>
 __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void k_attn(AttnArgs a) {
     using Pair = typename std::conditional<INT4, PairI4<HD>, PairF16<HD>>::type;
@@ -398,6 +401,7 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
     __shared__ __align__(16) float lds[kWaves * kRec];
     __shared__ h8_t qops[HD / 32 * kWave];
     __shared__ float qscale[kHeadsPerBlock];
+    __shared__ float2 norm[kHeadsPerBlock];  // without a join: a head's M (NaN: refused) and 1 / L
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, t = lane & 15;
     const int split = blockIdx.x, kvh = blockIdx.y / a.plan.groups, grp = blockIdx.y % a.plan.groups, b = blockIdx.z;
@@ -513,22 +517,27 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
         } else {  // the one block of its kv head
             const float il = no ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
             store_out(out + x, acc * il);
+            if (ACC && x % HD == 0) norm[h] = make_float2(no ? __builtin_nanf("") : M - kUp, il);
+        }
+    }
+    if constexpr (ACC) {
+        if (a.plan.join) return;
+        __syncthreads();
+        if (norm[0].x != norm[0].x) return;
+        const float* raw = a.raw + ((size_t)b * a.hq + h0) * cap;
+        float* weights = a.weights + ((size_t)b * a.hkv + kvh) * cap;
+        for (int s = threadIdx.x; s < ctx; s += kThreads) {
+            float acc = 0.0f;
+#pragma unroll
+            for (int h = 0; h < kHeadsPerBlock; ++h)
+                if (h < H) acc += part_of(raw[(size_t)h * cap + s], norm[h]);
+            weights[s] += acc;
         }
     }
 }
 
-// Blocks of a kernel that a compute unit holds at once.
-template <int HD, bool INT4, bool ACC>
-int blocks_per_cu() {
-    static const int n = [] {
-        int v = 0;
-        return hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, k_attn<HD, INT4, ACC>, kThreads, 0) == hipSuccess && v > 0 ? v : 1;
-    }();
-    return n;
-}
-
 // ------------------------------------------------------------------- k_join --
-// With weights.  The first `outs` blocks of a (kv head, sequence) merge the
+// The first `outs` blocks of a (kv head, sequence) merge the
 // records into 32 float4 columns of the output each, eight threads to a column;
 // the others turn 256 slots' scores into weights at a time.
 constexpr int kJoinThreads = 256, kJoinCols = 32;
@@ -536,7 +545,8 @@ constexpr int kJoinHeads = 64;  // query heads of a kv head
 
 template <int HD>
 __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int outs) {
-    __shared__ float fac[kJoinHeads * kMaxSplits], top[kJoinHeads], inv[kJoinHeads];
+    __shared__ float fac[kJoinHeads * kMaxSplits];
+    __shared__ float2 norm[kJoinHeads];
     __shared__ f4_t sums[kJoinThreads];
     __shared__ int refused;
     const int kvh = blockIdx.y, b = blockIdx.z, G = a.hq / a.hkv, ns = a.plan.splits, tid = threadIdx.x, rec = a.plan.rec;
@@ -584,8 +594,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int outs) {
             const float il = no ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
             if (lane < ns) fac[h * kMaxSplits + lane] = no ? il : e * il;
             if (lane == 0) {
-                top[h] = M - kUp;
-                inv[h] = il;
+                norm[h] = make_float2(M - kUp, il);
                 if (no) refused = 1;
             }
         }
@@ -608,19 +617,18 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int outs) {
     }
     if (refused) return;
     const int ctx = a.lens[b], stride = ((int)gridDim.x - outs) * kJoinThreads;
-    auto part_of = [&](float x, int h) { return __builtin_amdgcn_exp2f(x - top[h]) * inv[h]; };
     if (slot < ctx) {
         float acc = 0.0f;
 #pragma unroll
         for (int h = 0; h < 8; ++h)
-            if (h < G) acc += part_of(early[h], h);
-        for (int h = 8; h < G; ++h) acc += part_of(raw[(size_t)h * cap + slot], h);
+            if (h < G) acc += part_of(early[h], norm[h]);
+        for (int h = 8; h < G; ++h) acc += part_of(raw[(size_t)h * cap + slot], norm[h]);
         weights[slot] = was + acc;
     }
     for (int64_t s = (int64_t)slot + stride; s < ctx; s += stride) {
         float acc = 0.0f;
 #pragma unroll 8
-        for (int h = 0; h < G; ++h) acc += part_of(raw[(size_t)h * cap + s], h);
+        for (int h = 0; h < G; ++h) acc += part_of(raw[(size_t)h * cap + s], norm[h]);
         weights[s] += acc;
     }
 }
@@ -639,11 +647,6 @@ hipError_t attn_case(const AttnArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <bool INT4, bool ACC>
-int held(int hd) {
-    return hd == 64 ? blocks_per_cu<64, INT4, ACC>() : hd == 128 ? blocks_per_cu<128, INT4, ACC>() : blocks_per_cu<256, INT4, ACC>();
-}
-
 // The part of a plan that the heads decide.
 AttnPlan heads_plan(int hq, int hkv, int hd) {
     const int G = hq / hkv, heads = std::min(G, kHeadsPerBlock);
@@ -655,21 +658,31 @@ AttnPlan heads_plan(int hq, int hkv, int hd) {
 AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4, bool weights) {
     AttnPlan p = heads_plan(hq, hkv, hd);
     const int pairs = (max_blocks + 1) / 2;
-    // Blocks run in rounds of as many as the device holds at once; a round
-    // takes the time of a wavefront's pairs and, before and after them, of about
-    // two more (8 fp16 sequences of 4K: 26 us in one round of 256 blocks, 27.5 in
-    // two).  Fewer splits among equals: fewer records.
-    const int64_t rows = (int64_t)batch * hkv * p.groups;
-    const int64_t room = (int64_t)device_cus() * (int4 ? weights ? held<true, true>(hd) : held<true, false>(hd) : held<false, true>(hd));
+    // The splits of the least time, in steps of 10 ns, from sweeps over 1 to 64
+    // splits of contexts of 100 to 16384: 2.1 us for the launch; 1 us for each
+    // block that a compute unit gets, and for eight pairs of it 0.8 us (int4) or
+    // 1.4 us (fp16) per 64 dimensions, 15 % less where it holds two blocks at
+    // once, 0.4 of that and up for fewer than eight pairs; 3 us and a little per
+    // split for records and join, or without a join half a microsecond for eight
+    // pairs' weights.  (8 kv heads of 128, int4: 512 tokens 6.6 us in one block
+    // each and 7.7 in eight with a join, 1024 tokens 9.7 and 7.9; 8 sequences of
+    // 8192 21.2 us in four, 18.9 in eight; 6 of 2500, 8 heads of 64, fp16: 11.0 us
+    // in four, 11.9 in ten.)
+    const int64_t rows = (int64_t)batch * hkv * p.groups, cus = device_cus(), pair = (int4 ? 80 : 140) * (hd / 64);
+    const bool joined = weights && p.groups > 1, two = hd * (int4 ? 1 : 2) <= 128;
     int64_t least = INT64_MAX;
-    for (int s = 1; s <= kMaxSplits && (s == 1 || s <= (pairs + kWaves - 1) / kWaves); ++s) {
-        const int64_t cost = ((rows * s + room - 1) / room) * ((pairs + s * kWaves - 1) / (s * kWaves) + 2);
+    for (int s = 1; s <= std::min(kMaxSplits, pairs); ++s) {
+        const bool join = s > 1 || joined;
+        const int64_t of = (pairs + s - 1) / s, blocks = (rows * s + cus - 1) / cus;  // pairs of a block, blocks of a compute unit
+        const int64_t busy = of <= 4 ? 16 + 3 * of : of < 8 ? 24 + 2 * of : 5 * of;     // 40: eight pairs
+        const int64_t block = 100 + pair * busy * (two && blocks > 1 ? 17 : 20) / 800 + (weights && !join ? 50 * of / 8 : 0);
+        const int64_t cost = 210 + blocks * block + (join ? 300 + 3 * s : 0);
         if (cost < least) {
             least = cost;
             p.splits = s;
         }
     }
-    p.join = weights || p.splits > 1;
+    p.join = p.splits > 1 || joined;
     return p;
 }
 

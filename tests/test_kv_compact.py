@@ -461,9 +461,9 @@ def test_attention_int4_without_weights(ctx, hq, hkv, hd, lens):
 @pytest.mark.gpu
 @pytest.mark.parametrize("int4,weights", [(True, True), (True, False), (False, True)], ids=["int4", "int4-plain", "f16"])
 def test_attention_of_many_rows(ctx, int4, weights):
-    """More rows than the device holds blocks, so one block to a row, and one
-    long sequence among short ones: a wavefront's pages pass 64 of the table."""
-    check_attention(ctx, int4, 256, 4, 64, [9001] + [1, 17, 0, 40] * 47, weights=weights, nblk=1100)
+    """More rows than the device holds blocks, so one block to a row or two, and
+    one long sequence among short ones: a wavefront's pages pass 64 of the table."""
+    check_attention(ctx, int4, 256, 4, 64, [18001] + [1, 17, 0, 40] * 47, weights=weights, nblk=1500)
 
 
 @pytest.mark.gpu
