@@ -5,13 +5,14 @@
 // kv head for up to 8 of its query heads, keeps an online softmax per head,
 // merges its wavefronts through LDS and writes one record (O, M, L), or the
 // fp16 output where it has the kv head to itself.  With weights it also writes
-// the scores, and with the kv head to itself it adds the weights as well.  k_join: merges the records and, with weights, turns the scores
-// into exp(s - M) / L, whose sum over the query heads of the kv head it adds to
-// the weights.  (The scores need M and L of all splits, which no block of k_attn
-// has; reading them back costs 8 bytes a token and query head, the pages again
-// would cost 9/16 byte or more a value.  Merging the records in the last block of
-// k_attn instead took as long for 8 splits and longer for more: 18.3 against
-// 15.5 us for 64.)
+// the scores, and with the kv head to itself it adds the weights as well.
+// k_join: merges the records and, with weights, turns the scores into exp(s - M)
+// / L, whose sum over the query heads of the kv head it adds to the weights.
+// (The scores need M and L of all splits, which no block of k_attn has; reading
+// them back costs 8 bytes a token and query head, the pages again would cost
+// 9/16 byte or more a value.  Merging the records in the last block of k_attn
+// instead took as long for 8 splits and longer for more: 18.3 against 15.5 us
+// for 64.)
 //
 // Products are v_mfma_f32_16x16x32_f16 (A: lane l holds row l%16, k = 8 (l/16)
 // .. +7; B: column l%16, the same k; C: column l%16, rows 4 (l/16) .. +3).
