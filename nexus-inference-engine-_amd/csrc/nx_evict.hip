@@ -411,7 +411,7 @@ __device__ inline void move_f16(const EvictArgs& a, int part, size_t dst, size_t
         for (int i = 0; i < KN; ++i) {
             const int t = i * KT + lane / KL;
             const size_t p = __shfl(src, t, kWave) + 2 * HD * __shfl(u, t, kWave);
-            if (moved >> t & 1u) k[i] = reinterpret_cast<const u4_t*>(a.kpool + p)[lane % KL];
+            if (moved >> t & 1u) k[i] = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(a.kpool + p) + lane % KL);
         }
 #pragma unroll
         for (int i = 0; i < KN; ++i) {
