@@ -511,7 +511,7 @@ __device__ inline void move_int4(const EvictArgs& a, size_t dst, size_t src, int
 // token leaves is cleared by the lane that has read it, every other by its own.
 // fp16: bound by memory, since V's pages are dimension-major, so that a token
 // moves with whole pages: 8 sequences of 8192 tokens of 8 kv heads of 128 cut to
-// 2048 read 169 MB and write 66, 54 us; int4, one of 32768 cut to 4096: 8 us.
+// 2048 read 173 MB and write 65, 53 us; int4, one of 32768 cut to 4096: 7.7 us.
 template <int HD, bool INT4>
 constexpr int kParts = INT4 ? 1 : 1 + HD / kWave;  // wavefronts of a page
 
