@@ -123,9 +123,24 @@ __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
     const size_t at = ((size_t)b * a.hkv + h) * cap;
     const float* w_in = a.weights_in + at;
     const int32_t* t_in = a.tags_in + at;
-    // the table's entries are requested here and looked at behind the first loop
+    // The first weights and tags are requested ahead of the lengths, as those of a
+    // row that fills its slots (most often right where rows are cut), and the
+    // table's entries, which are looked at behind the first loop.
+    float w[8];
+    int t[8];
+    const int guess = (cap + kPickThreads - 1) / kPickThreads;
+    auto request_upto = [&](int s, int last) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = w_in[min(s + j * kWave, last)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = t_in[min(s + j * kWave, last)];
+    };
+    request_upto(wave * guess * kWave + lane, cap - 1);
     const int32_t* table = a.table + (size_t)b * a.max_blocks;
     const int entry[2] = {table[min(tid, a.max_blocks - 1)], table[min(tid + kPickThreads, a.max_blocks - 1)]};
+    for (int i = tid; i < kBins; i += kPickThreads) hist[i] = make_uint2(0u, 0u);
+    if (tid == 0) listed = 0;
+    asm volatile("" ::: "memory");  // (all of this before the wait for the lengths)
     bool bad = L < 0 || L > cap || N < L;
     const int pages = bad ? 0 : (L + kPage - 1) / kPage, ahead = (int)((unsigned)N - (unsigned)L + 1u);
     auto outside = [&] {
@@ -139,8 +154,6 @@ __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
         if (tid == 0 && h == 0) *seq_of(a, b) = {bad ? -1 : L, 0, ahead};
         return;
     }
-    for (int i = tid; i < kBins; i += kPickThreads) hist[i] = make_uint2(0u, 0u);
-    if (tid == 0) listed = 0;
     __syncthreads();
     uint32_t* keys;
     if constexpr (SLOTS > 0)
@@ -178,36 +191,21 @@ __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
     };
     // eight steps at a time, the next eight requested ahead; then the last few
     const int full = max(s1 - s0, 0) / (8 * kWave) * 8;
-    float w[8];
-    int t[8];
-    if (full > 0) {
-        auto request = [&](int u) {
-            const float* wp = w_in + s0 + u * kWave + lane;
-            const int32_t* tp = t_in + s0 + u * kWave + lane;
+    if (steps != guess && mine_n > 0) request_upto(s0 + lane, s1 - 1);
+    for (int u0 = 0; u0 < full; u0 += 8) {
+        const int s = s0 + u0 * kWave + lane, next = s0 + min(u0 + 8, full - 8) * kWave + lane;
+        uint32_t key[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j] = wp[j * kWave];
-                t[j] = tp[j * kWave];
-            }
-        };
-        request(0);
-        for (int u0 = 0; u0 < full; u0 += 8) {
-            const int s = s0 + u0 * kWave + lane;
-            uint32_t key[8];
+        for (int j = 0; j < 8; ++j) key[j] = key_of(s + j * kWave, w[j], t[j]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) key[j] = key_of(s + j * kWave, w[j], t[j]);
-            request(min(u0 + 8, full - 8));
+        for (int j = 0; j < 8; ++j) w[j] = w_in[next + j * kWave];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) put(s + j * kWave, key[j]);
-        }
+        for (int j = 0; j < 8; ++j) t[j] = t_in[next + j * kWave];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) put(s + j * kWave, key[j]);
     }
     if (full < mine_n) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int s = min(s0 + (full + j) * kWave + lane, s1 - 1);
-            w[j] = w_in[s];
-            t[j] = t_in[s];
-        }
+        if (full > 0) request_upto(s0 + full * kWave + lane, s1 - 1);
         uint32_t key[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
