@@ -24,7 +24,10 @@
 //
 // int4-g32: a step of 32 dimensions is one scale group, so codes enter the
 // products as exact fp16 integers and the scales stay outside: fp32 behind K's
-// product, in front of V's with the probability.
+// product, in front of V's with the probability.  Bound by the vector
+// instructions beside the products (about 300 a pair of pages of 128 dimensions)
+// and, one pair to a wavefront, by latency: 32768 tokens of 8 kv heads (38 MB)
+// 11.4 us and a join of 3.9.
 #include <algorithm>
 #include <type_traits>
 
@@ -174,17 +177,30 @@ __device__ inline h8_t codes8(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(h8_t, H2x4{low_codes(a), high_codes(a), low_codes(b), high_codes(b)});
 }
 
+// K's codes as they are: a nibble in the last bits of a half is the subnormal
+// number code 2^-24, in the next four code 2^-20, and the products take both
+// exactly, so a mask is all that a pair of codes takes.  q's dimensions 2, 3, 6
+// and 7 of eight are 1/16 of what they were, and a product begins at -8 times
+// q's sum over its 32 dimensions.  (V's cannot go so: what taking off 8 p leaves,
+// 2^-21 of a scale, would stand where every value is 0.)
+struct W4 {
+    uint32_t w[4];
+};
+__device__ inline h8_t raw_codes8(uint32_t w) {
+    return __builtin_bit_cast(h8_t, W4{w & 0x000F000Fu, w & 0x00F000F0u, w >> 8 & 0x000F000Fu, w >> 8 & 0x00F000F0u});
+}
+
 // ------------------------------------------------------------ scores of a pair --
 template <int HD>
-__device__ inline void scores(const PairI4<HD>& r, const h8_t* q, f4_t (&s)[2]) {
+__device__ inline void scores(const PairI4<HD>& r, const h8_t* q, const f4_t* off, f4_t (&s)[2]) {
     s[0] = s[1] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
         const h8_t qi = q[i * kWave];
+        const f4_t o = off[i * 16];
 #pragma unroll
         for (int pg = 0; pg < 2; ++pg) {
-            const h8_t k = codes8(r.k[pg][i], r.k[pg][i] >> 8);
-            const f4_t d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qi, f4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            const f4_t d = __builtin_amdgcn_mfma_f32_16x16x32_f16(raw_codes8(r.k[pg][i]), qi, o, 0, 0, 0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[pg][j] = __builtin_fmaf(d[j], (float)r.ks[pg][i][j], s[pg][j]);
         }
@@ -193,7 +209,7 @@ __device__ inline void scores(const PairI4<HD>& r, const h8_t* q, f4_t (&s)[2]) 
 }
 
 template <int HD>
-__device__ inline void scores(const PairF16<HD>& r, const h8_t* q, f4_t (&s)[2]) {
+__device__ inline void scores(const PairF16<HD>& r, const h8_t* q, const f4_t*, f4_t (&s)[2]) {
     s[0] = s[1] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
@@ -303,7 +319,7 @@ __device__ inline void values(const PairF16<HD>& r, const float (&p)[8], f4_t (&
 // part.  A power of two per head brings its largest value to 512 and up, so
 // that low parts are normal fp16 numbers and no high part overflows; scale[t]
 // takes it back.
-template <int HD>
+template <int HD, bool INT4>
 struct StageQ {
     static constexpr int T = HD / 4;  // threads of a head, four dimensions each
     static_assert(T * kHeadsPerBlock <= kThreads && kWave % T == 0, "a head lies in one wavefront");
@@ -312,7 +328,7 @@ struct StageQ {
         const int h = threadIdx.x / T, d = 4 * (threadIdx.x % T);
         x = h < H ? *reinterpret_cast<const f4_t*>(q + (size_t)h * HD + d) : f4_t{0.f, 0.f, 0.f, 0.f};
     }
-    __device__ void store(_Float16* ops, float* scale) const {
+    __device__ void store(_Float16* ops, float* scale, f4_t* off) const {
         const int h = threadIdx.x / T, d = 4 * (threadIdx.x % T);
         if (h >= kHeadsPerBlock) return;
         float top = row16_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
@@ -321,16 +337,28 @@ struct StageQ {
         const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
         const int up = e == 0 || e == 255 ? 0 : min(136 - e, 126);
         h4_t hi, lo;
+        float sum[2] = {0.0f, 0.0f};  // of the parts, times -8 2^-24
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float y = ldexpf(x[j], up);
+            const float part = INT4 && j >= 2 ? 0.0625f : 1.0f, y = ldexpf(x[j], up) * part;  // (raw_codes8)
             hi[j] = (_Float16)y;
             lo[j] = (_Float16)(y - (float)hi[j]);
+            sum[0] = __builtin_fmaf((float)hi[j], -0x1p-21f / part, sum[0]);
+            sum[1] = __builtin_fmaf((float)lo[j], -0x1p-21f / part, sum[1]);
         }
+        if (INT4)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v = sum[i] + dpp<kQuadXor1>(sum[i]);
+                v += dpp<kQuadXor2>(v);
+                v += dpp<kRowHalfMirror>(v);
+                if (d % 32 == 0) off[d / 32 * 16 + h + 8 * i] = f4_t{v, v, v, v};
+            }
         const int at = ((d / 32) * kWave + 16 * (d % 32 / 8)) * 8 + d % 8;
         *reinterpret_cast<h4_t*>(ops + at + 8 * h) = hi;
         *reinterpret_cast<h4_t*>(ops + at + 8 * (h + 8)) = lo;
-        if (d == 0) scale[h] = ldexpf(kLog2e / sqrtf((float)HD), -up);
+        // codes enter as code 2^-24 (2^120 at most: scores of such a q are far apart anyway)
+        if (d == 0) scale[h] = ldexpf(kLog2e / sqrtf((float)HD), INT4 ? min(24 - up, 120) : -up);
     }
 };
 
@@ -338,10 +366,10 @@ struct StageQ {
 // one's has become scores, its V once this one's is added: half a pair is in
 // flight all the time, in registers that are free anyway.
 template <int HD, bool ACC, class Pair, class Next>
-__device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, float scale, int na, int nb, float* raw, int lane, Next next_k) {
+__device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, const f4_t* off, float scale, int na, int nb, float* raw, int lane, Next next_k) {
     const int g = lane >> 4;
     f4_t s[2];
-    scores<HD>(r, q, s);
+    scores<HD>(r, q, off, s);
     // (here, not after the next request, whose registers these were)
     asm volatile("" : "+v"(s[0]), "+v"(s[1]));
     next_k();
@@ -404,6 +432,7 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
     __shared__ __align__(16) float lds[kWaves * kRec];
     __shared__ h8_t qops[HD / 32 * kWave];
     __shared__ float qscale[kHeadsPerBlock];
+    __shared__ f4_t qoff[INT4 ? HD / 32 * 16 : 1];  // what K's products begin at
     __shared__ float2 norm[kHeadsPerBlock];  // without a join: a head's M (NaN: refused) and 1 / L
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, t = lane & 15;
@@ -413,7 +442,7 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
     const int stride = a.plan.splits * kWaves, first = split + a.plan.splits * wave;
     // q and the table entries of the first 32 pairs (two lanes each) are
     // requested with the length, not behind it
-    StageQ<HD> stage;
+    StageQ<HD, INT4> stage;
     stage.request(a.q + ((size_t)b * a.hq + h0) * HD, H);
     const int32_t* table = a.table + (size_t)b * a.max_blocks;
     auto entry_of = [&](int i) {
@@ -444,10 +473,11 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
         turn_to(0);
         load_k<HD>(r, a, blk, kvh, lane);
     }
-    stage.store(reinterpret_cast<_Float16*>(qops), qscale);
+    stage.store(reinterpret_cast<_Float16*>(qops), qscale, qoff);
     __syncthreads();
     if (mine > 0) load_v<HD>(r, a, blk, kvh, lane);
     const h8_t* q = qops + lane;
+    const f4_t* off = qoff + t;
     const float scale = qscale[t & 7];
     Fold<HD> f;
 #pragma unroll
@@ -455,7 +485,7 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
     auto use = [&](int i, auto next_k) {
         const int page = 2 * (first + stride * i);
         float* raw = ACC && t < H ? a.raw + ((size_t)b * a.hq + h0 + t) * cap + page * kPage + 4 * g : nullptr;
-        fold<HD, ACC>(f, r, q, scale, min(ctx - page * kPage, kPage), min(max(ctx - (page + 1) * kPage, 0), kPage), raw, lane, next_k);
+        fold<HD, ACC>(f, r, q, off, scale, min(ctx - page * kPage, kPage), min(max(ctx - (page + 1) * kPage, 0), kPage), raw, lane, next_k);
     };
     // (the last pair apart: a request that may not come makes the waits for
     // others wait for all)

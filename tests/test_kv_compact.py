@@ -4,7 +4,7 @@ plain numpy forms in 64 bits written here from the definitions; codes, moved
 tokens, tags and lengths bit for bit.
 
 Tolerances count roundings.  With A = sum_t p_t |v_t| of an output element:
-  scores    q enters as fp16 hi + lo (2^-22 of q, 2^-34 of the head's largest), products add in fp32, and
+  scores    q enters as fp16 hi + lo (2^-22 of q, 2^-30 of the head's largest), products add in fp32, and
             1/sqrt(hd) log2(e) is one more rounding: at most
             es = (hd + 32) 2^-24 max_t sum_i |q_i k_i| / sqrt(hd) each way
   weights   p is off by at most e = 2 es + 2^-19 of itself (exp2 and its
