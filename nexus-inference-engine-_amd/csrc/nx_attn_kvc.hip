@@ -46,7 +46,7 @@ constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kMaxSplits = 64;
 constexpr int kRowRor8 = 0x128;
-constexpr float kUp = 11.0f, kLead = 4.0f;
+constexpr float kUp = 11.0f, kLead = 4.0f, kFar = 1048576.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Lane l's and lane l ^ 16's (32's) larger value, and their sum.
@@ -390,14 +390,24 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, const f4_t* off
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, p[j]);
     top = max_x32(max_x16(top)) * scale;  // over the column's four lanes
-    const float mn = top > f.m + kLead ? top : f.m;
+    // Far from 0 (kFar) a step of the scores' 24 bits is near the powers of two
+    // that p has to spare: there they are rounded and taken from the maximum
+    // itself before anything is added.
+    const bool far = __any(fabsf(top) > kFar);
+    const float mn = top > (far ? f.m : f.m + kLead) ? top : f.m;
     const bool none = mn == -__builtin_inff();  // no token, or NaN scores alone
     const float up = most_up<HD>(r, f.up);
-    const float corr = none ? 1.0f : __builtin_amdgcn_exp2f(f.m - mn + (up - f.up)), from = none ? 0.0f : mn - up;
-    float sum = 0.0f;
+    const float corr = none ? 1.0f : __builtin_amdgcn_exp2f(f.m - mn + (up - f.up));
+    float by = scale, from = none ? 0.0f : mn - up, sum = 0.0f;
+    if (far) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = p[j] * scale - (none ? 0.0f : mn);
+        by = 1.0f;
+        from = none ? 0.0f : -up;
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], scale, -from));
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j], by, -from));
         sum += p[j];
     }
     f.l = f.l * corr + sum;
@@ -423,7 +433,7 @@ __device__ inline void store_out(uint16_t* out, f4_t v) {
 }
 
 // The weight of a score, from its head's M and 1 / L.
-__device__ inline float part_of(float score, float2 norm) { return __builtin_amdgcn_exp2f(score - norm.x) * norm.y; }
+__device__ inline float part_of(float score, float2 norm) { return __builtin_amdgcn_exp2f(score - norm.x + kUp) * norm.y; }
 
 template <int HD, bool INT4, bool ACC>
 __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void k_attn(AttnArgs a) {
@@ -550,7 +560,7 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
         } else {  // the one block of its kv head
             const float il = no ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
             store_out(out + x, acc * il);
-            if (ACC && x % HD == 0) norm[h] = make_float2(no ? __builtin_nanf("") : M - kUp, il);
+            if (ACC && x % HD == 0) norm[h] = make_float2(no ? __builtin_nanf("") : M, il);
         }
     }
     if constexpr (ACC) {
@@ -627,7 +637,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(AttnArgs a, int outs) {
             const float il = no ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
             if (lane < ns) fac[h * kMaxSplits + lane] = no ? il : e * il;
             if (lane == 0) {
-                norm[h] = make_float2(M - kUp, il);
+                norm[h] = make_float2(M, il);
                 if (no) refused = 1;
             }
         }

@@ -490,6 +490,31 @@ def test_attention_peaked_rows_and_calls_in_a_row(ctx, int4):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("int4", [True, False], ids=["int4", "f16"])
+@pytest.mark.parametrize("qamp", [0.0, 1e-42, 1e-30, 1e30, 3e37])
+def test_attention_extreme_queries(ctx, int4, qamp):
+    """Queries far below and above 1: all tokens weigh the same, or one weighs 1
+    (p is exact then, so an output is off by the rounding of p times the scale
+    and its own, 2^-11 of it each)."""
+    rng = np.random.default_rng(12)
+    hq, hkv, hd, n, mb = 4, 2, 64, 50, 4
+    kp, vp, k64, v64, table = cache(rng, int4, [n], hkv, hd, mb, mb)
+    q = (rng.uniform(-1, 1, (1, hq, hd)) * qamp).astype(np.float32)
+    h = Held(ctx, q=q, kp=kp, vp=vp, table=table, lens=np.array([n], np.int32), out=np.zeros((1, hq, hd), np.float16),
+             w=np.zeros((1, hkv, mb * PAGE), np.float32))
+    f = ctx.attn_decode_paged_int4 if int4 else ctx.attn_decode_paged_f16_acc
+    f(h["q"], h["kp"], h["vp"], h["table"], h["lens"], h["out"], h["w"], 1, hq, hkv, hd, mb, mb)
+    out, w = h.get("out")[0].astype(np.float64), h.get("w")[0]
+    h.free()
+    want, W, A, e = attention(q[0], in_order(k64, table[0], n), in_order(v64, table[0], n))
+    if qamp > 1:
+        assert np.array_equal(W, np.round(W)) and np.array_equal(w[:, :n], W)
+        e = 0.0
+    assert (np.abs(out - want) <= 2.0**-11 * (np.abs(want) + A) + (e + 2.0**-19) * A + 2.0**-25).all()
+    assert np.abs(w[:, :n] - W).max() <= e * W.max() + 2.0**-22
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int4", [True, False], ids=["int4", "f16"])
 def test_attention_out_of_range(ctx, int4):
     """A length or a table entry out of range: NaN rows, weights as they were,
     the other sequences unharmed."""
