@@ -7,8 +7,8 @@
 // the rows with the table entry, which they do not depend on, K's with V's.  K
 // codes leave the threads as the dwords of their page, V codes, whose dwords
 // hold four tokens each, cross through LDS.  8192 tokens of 8 kv heads of 128
-// (76 MB): 18.6 us in and 16.6 us out by turns, when each waits for the other's
-// rows to leave the caches.
+// (76 MB): 18 us in and 13 us out by turns, when each waits for the other's rows
+// to leave the caches.
 #include "nx_kvc.h"
 
 namespace nx {
@@ -142,26 +142,42 @@ __global__ __launch_bounds__(2 * HD) void k_append_int4(RowArgs a) {
         words[tid] = (words[tid] & ~mask) | out;
 }
 
+// Four values to a thread of each of two tokens, so that a store's lanes write
+// whole lines (with eight of one token 4096 tokens took 14.0 us in place of 12.3).
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void k_read_int4(RowArgs a) {
-    constexpr int S = HD / 32, C = HD / 8;
+    constexpr int S = HD / 32, C = HD / 4;
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const RowPage pr = row_page(a.start[b], a.tokens, a.max_blocks, blockIdx.x);
     if (pr.none) return;
-    const int t = tid / C, c = tid % C, row = pr.row0 + t;
-    const bool have = row >= 0 && row < a.tokens;
-    const size_t at = have ? (((size_t)b * a.tokens + row) * a.hkv + h) * HD + 8 * c : 0;
+    const int c = tid % C, t0 = tid / C;
+    bool have[2];
+    size_t at[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int row = pr.row0 + t0 + 8 * u;
+        have[u] = row >= 0 && row < a.tokens;
+        at[u] = have[u] ? (((size_t)b * a.tokens + row) * a.hkv + h) * HD + 4 * c : 0;
+    }
     const int64_t rec = page_record<HD>(a, pr, b, h);
     if (rec < 0) {
         const float nan = __builtin_nanf("");
-        if (have)
-            for (float* p : {a.k + at, a.v + at})
-                for (int j = 0; j < 2; ++j) reinterpret_cast<f4_t*>(p)[j] = f4_t{nan, nan, nan, nan};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (have[u])
+                for (float* p : {a.k + at[u], a.v + at[u]}) *reinterpret_cast<f4_t*>(p) = f4_t{nan, nan, nan, nan};
         return;
     }
-    const int sat = scale_at(HD, t, c / 4);
-    const uint16_t s16[2] = {reinterpret_cast<const uint16_t*>(a.kpool + rec + 8 * HD)[sat], reinterpret_cast<const uint16_t*>(a.vpool + rec + 8 * HD)[sat]};
-    const uint32_t wk = reinterpret_cast<const uint32_t*>(a.kpool + rec)[k_word(HD, t, 8 * c)], wv = reinterpret_cast<const uint32_t*>(a.vpool + rec)[tid];
+    const uint32_t wv = reinterpret_cast<const uint32_t*>(a.vpool + rec)[tid];
+    uint16_t s16[2][2];
+    uint32_t wk[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int t = t0 + 8 * u, sat = scale_at(HD, t, c / 8);
+        s16[u][0] = reinterpret_cast<const uint16_t*>(a.kpool + rec + 8 * HD)[sat];
+        s16[u][1] = reinterpret_cast<const uint16_t*>(a.vpool + rec + 8 * HD)[sat];
+        wk[u] = reinterpret_cast<const uint32_t*>(a.kpool + rec)[k_word(HD, t, 4 * c)] >> (c % 2 * 8);
+    }
     __shared__ uint8_t codes[kPage * HD];
     const int i = tid % S, n = (tid / S) % 16, g = tid / S / 16, d = 32 * i + n;
 #pragma unroll
@@ -169,18 +185,19 @@ __global__ __launch_bounds__(2 * HD) void k_read_int4(RowArgs a) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) codes[(4 * g + j) * HD + d + 16 * e] = (uint8_t)((wv >> (4 * v_nib(j, 16 * e))) & 15u);
     __syncthreads();
-    if (!have) return;
-    const uint2 q = *reinterpret_cast<const uint2*>(codes + t * HD + 8 * c);
-    f4_t k[2], v[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        k[j / 4][j % 4] = (float)((int)((wk >> (4 * k_nib(j))) & 15u) - 8) * h2f_bits(s16[0]);
-        v[j / 4][j % 4] = (float)((int)(((j < 4 ? q.x : q.y) >> (8 * (j % 4))) & 255u) - 8) * h2f_bits(s16[1]);
-    }
+    for (int u = 0; u < 2; ++u) {
+        const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + (t0 + 8 * u) * HD + 4 * c);
+        f4_t k, v;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        reinterpret_cast<f4_t*>(a.k + at)[j] = k[j];
-        reinterpret_cast<f4_t*>(a.v + at)[j] = v[j];
+        for (int j = 0; j < 4; ++j) {  // (dimensions 4 .. 7 of eight lie one byte on)
+            k[j] = (float)((int)((wk[u] >> (4 * k_nib(j))) & 15u) - 8) * h2f_bits(s16[u][0]);
+            v[j] = (float)((int)((q >> (8 * j)) & 255u) - 8) * h2f_bits(s16[u][1]);
+        }
+        if (have[u]) {
+            *reinterpret_cast<f4_t*>(a.k + at[u]) = k;
+            *reinterpret_cast<f4_t*>(a.v + at[u]) = v;
+        }
     }
 }
 
