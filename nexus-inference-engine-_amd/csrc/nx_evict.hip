@@ -418,24 +418,31 @@ __device__ inline void move_f16(const EvictArgs& a, int part, size_t dst, size_t
         }
         return;
     }
-    // a dimension's 16 tokens a lane, written as one row
-    const int d = (part - 1) * kWave + lane;
-    uint16_t v[kPage] = {};
+    // Half a dimension's row (eight tokens) a lane, of dimensions r and r + 32: a
+    // store's lanes write whole lines.
+    const int half = lane & 1, r = (part - 1) * kWave + lane / 2;
+    const unsigned mine = moved >> (8 * half) & 0xFFu;
+    uint16_t v[8][2] = {};
     u4_t row[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) row[j] = reinterpret_cast<const u4_t*>(a.vpool + dst)[2 * d + j];
+    for (int i = 0; i < 2; ++i) row[i] = reinterpret_cast<const u4_t*>(a.vpool + dst)[2 * (r + 32 * i) + half];
 #pragma unroll
-    for (int t = 0; t < kPage; ++t)
-        if (moved >> t & 1u)
-            v[t] = (reinterpret_cast<const uint16_t*>(a.vpool + lane64(src, t)) + __builtin_amdgcn_readlane(u, t))[(uint32_t)d * kPage];
+    for (int k = 0; k < 8; ++k) {
+        if (!(moved >> k & 0x101u)) continue;
+        const size_t from = (half ? lane64(src, 8 + k) : lane64(src, k)) + 2 * (half ? __builtin_amdgcn_readlane(u, 8 + k) : __builtin_amdgcn_readlane(u, k));
+        if (mine >> k & 1u)
 #pragma unroll
-    for (int t = 0; t < kPage; ++t)
-        if (moved >> t & 1u) {
-            const uint32_t w = row[t / 8][t / 2 % 4];
-            row[t / 8][t / 2 % 4] = t % 2 ? (w & 0xFFFFu) | (uint32_t)v[t] << 16 : (w & 0xFFFF0000u) | v[t];
+            for (int i = 0; i < 2; ++i) v[k][i] = reinterpret_cast<const uint16_t*>(a.vpool + from)[(uint32_t)(r + 32 * i) * kPage];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t w = row[i][k / 2], x = k % 2 ? (w & 0xFFFFu) | (uint32_t)v[k][i] << 16 : (w & 0xFFFF0000u) | v[k][i];
+            row[i][k / 2] = mine >> k & 1u ? x : w;
         }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) reinterpret_cast<u4_t*>(a.vpool + dst)[2 * d + j] = row[j];
+        reinterpret_cast<u4_t*>(a.vpool + dst)[2 * (r + 32 * i) + half] = row[i];
+    }
 }
 
 template <int HD>
@@ -509,7 +516,7 @@ __device__ inline void move_int4(const EvictArgs& a, size_t dst, size_t src, int
 // token leaves is cleared by the lane that has read it, every other by its own.
 // fp16: bound by memory, since V's pages are dimension-major, so that a token
 // moves with whole pages: 8 sequences of 8192 tokens of 8 kv heads of 128 cut to
-// 2048 read 173 MB and write 65, 53 us; int4, one of 32768 cut to 4096: 7.7 us.
+// 2048 read 173 MB and write 65, 51.5 us; int4, one of 32768 cut to 4096: 7.7 us.
 template <int HD, bool INT4>
 constexpr int kParts = INT4 ? 1 : 1 + HD / kWave;  // wavefronts of a page
 
