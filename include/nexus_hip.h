@@ -232,8 +232,9 @@ nx_status nx_attn_decode_paged_tq(nx_ctx* ctx, nx_buf q_f32, nx_buf kc4, nx_buf 
                                   int batch, int hq, int hkv, int max_blocks, int num_blocks);
 /* ---- int4-g32 KV pages.  For a cache of 9/32 of fp16 pages' size with heads
  * of 64, 128 or 256.  These calls check lengths, positions and block tables
- * in their kernels: they do not wait for the device and may be captured into
- * a token batch; what a sequence out of range gets is said at each call.
+ * in their kernels: they do not wait for the device (but for a workspace that
+ * grows outside a token batch) and may be captured into a token batch; what a
+ * sequence out of range gets is said at each call.
  *
  * Append `tokens` rows per sequence, k and v fp32 [batch][tokens][hkv]
  * [head_dim]: row i of sequence b goes to position positions[b] + i through
