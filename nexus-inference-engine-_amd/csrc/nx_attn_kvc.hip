@@ -65,6 +65,12 @@ __device__ inline float sum_x32(float v) {
     const uint32_t x = a[0], y = a[1];
     return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
 }
+// Lower lanes: the sum of a's two halves, upper lanes: of b's.
+__device__ inline float halves_sum(float a, float b) {
+    const auto v = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t x = v[0], y = v[1];
+    return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+}
 __device__ inline float max_x32(float v) {
     const auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
     const uint32_t x = a[0], y = a[1];
@@ -155,6 +161,10 @@ __device__ inline void load_v(PairF16<HD>& r, const AttnArgs& a, const int (&blk
     }
 }
 
+struct H2x4 {
+    half2_t h[4];
+};
+
 // Codes of half a dword (nibbles 0 and 4, 1 and 5) as fp16 values code - 8:
 // 0x6400 is 1024, whose last bits a nibble sets; both steps are exact.
 __device__ inline uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
@@ -170,9 +180,6 @@ __device__ inline half2_t high_codes(uint32_t w) {  // 1024 + 16 code
     const half2_t v = __builtin_bit_cast(half2_t, and_or(w, 0x00F000F0u, 0x64006400u));
     return __builtin_elementwise_fma(v, half2_t{(_Float16)0.0625f, (_Float16)0.0625f}, half2_t{(_Float16)-72.0f, (_Float16)-72.0f});
 }
-struct H2x4 {
-    half2_t h[4];
-};
 __device__ inline h8_t codes8(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(h8_t, H2x4{low_codes(a), high_codes(a), low_codes(b), high_codes(b)});
 }
@@ -255,8 +262,7 @@ struct Fold {
 
 // ------------------------------------------------------------ values of a pair --
 // The powers of two that a pair's probabilities may have.  P V takes p
-// times the token's scale, rounded to fp16: at most 2^-11 of a term, which
-// stays linear in the output (an fp16 number itself).  With p up to 2^15 a
+// times the token's scale as fp16 numbers (below).  With p up to 2^15 a
 // scale of 2 or more (a value of 16 and up among a group) could pass the
 // largest fp16 number: from such a pair on the wavefront's factor is as many
 // powers of two smaller.
@@ -281,22 +287,44 @@ __device__ inline float most_up(const PairF16<HD>&, float up) {
     return up;
 }
 
+// The lanes of columns 8-15 (those with bit 3), which hold the same
+// probabilities as columns 0-7: rows 0-7 of a product take the fp16 high parts
+// of the heads' factors and rows 8-15 the low parts.
+__device__ inline bool low_part() { return __builtin_amdgcn_inverse_ballot_w64(0xFF00FF00FF00FF00ull); }
+
 // o += P V.  p: probabilities of tokens 4 g + j of page a (j < 4) and page b.
+// int4 pages: the factors are p times the token's scale.  The high part is the
+// rounded product of p's high part and the scale, the low part what that
+// rounding left out (exactly: one fused step) and the product with p's low
+// part, so both are 2^-21 of a factor, or fp16's smallest number.  (The high
+// part alone, 2^-11, is what an output rounds to, but of its terms'
+// magnitudes, not of their sum: it made outputs differ by 3e-4.)
 template <int HD>
 __device__ inline void values(const PairI4<HD>& r, const float (&p)[8], f4_t (&o)[HD / 16], int) {
+    H2x4 part, less;  // p's own part; in lanes of low parts p's high one, negative, else 0
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const half2_t hi = {(_Float16)p[2 * j], (_Float16)p[2 * j + 1]};
+        const half2_t lo = {(_Float16)(p[2 * j] - (float)hi.x), (_Float16)(p[2 * j + 1] - (float)hi.y)};
+        const uint32_t h = __builtin_bit_cast(uint32_t, hi), l = __builtin_bit_cast(uint32_t, lo);
+        part.h[j] = __builtin_bit_cast(half2_t, low_part() ? l : h);
+        less.h[j] = __builtin_bit_cast(half2_t, low_part() ? h ^ 0x80008000u : 0u);
+    }
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
-        h8_t ps;
+        const H2x4 vs = __builtin_bit_cast(H2x4, __builtin_shufflevector(r.vs[0][i], r.vs[1][i], 0, 1, 2, 3, 4, 5, 6, 7));
+        H2x4 ps;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ps[j] = (_Float16)__builtin_fmaf(p[j], (float)r.vs[j / 4][i][j % 4], 0.0f);
-        o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps, codes8(r.v[0][i], r.v[1][i]), o[2 * i], 0, 0, 0);
-        o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ps, codes8(r.v[0][i] >> 8, r.v[1][i] >> 8), o[2 * i + 1], 0, 0, 0);
+        for (int j = 0; j < 4; ++j)
+            ps.h[j] = __builtin_elementwise_fma(part.h[j], vs.h[j], __builtin_elementwise_fma(-less.h[j], vs.h[j], less.h[j] * vs.h[j]));
+        const h8_t a = __builtin_bit_cast(h8_t, ps);
+        o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, codes8(r.v[0][i], r.v[1][i]), o[2 * i], 0, 0, 0);
+        o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, codes8(r.v[0][i] >> 8, r.v[1][i] >> 8), o[2 * i + 1], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-// fp16 pages: rows 0-7 of the product take the fp16 high parts of the heads'
-// probabilities and rows 8-15 (the lanes of columns 8-15) the low parts.
+// fp16 pages: the factors are the probabilities themselves.
 template <int HD>
 __device__ inline void values(const PairF16<HD>& r, const float (&p)[8], f4_t (&o)[HD / 16], int lane) {
     const bool low = lane & 8;
@@ -485,7 +513,6 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
     }
     stage.store(reinterpret_cast<_Float16*>(qops), qscale, qoff);
     __syncthreads();
-    if (mine > 0) load_v<HD>(r, a, blk, kvh, lane);
     const h8_t* q = qops + lane;
     const f4_t* off = qoff + t;
     const float scale = qscale[t & 7];
@@ -498,32 +525,43 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
         fold<HD, ACC>(f, r, q, off, scale, min(ctx - page * kPage, kPage), min(max(ctx - (page + 1) * kPage, 0), kPage), raw, lane, next_k);
     };
     // (the last pair apart: a request that may not come makes the waits for
-    // others wait for all)
-    for (int i = 0; i + 1 < mine; ++i) {
-        use(i, [&] {
-            turn_to(i + 1);
-            load_k<HD>(r, a, blk, kvh, lane);
-        });
-        load_v<HD>(r, a, blk, kvh, lane);
+    // others wait for all; heads of 256 need one branch around all requests for
+    // that, which costs the others registers)
+    auto fold_all = [&] {
+        for (int i = 0; i + 1 < mine; ++i) {
+            use(i, [&] {
+                turn_to(i + 1);
+                load_k<HD>(r, a, blk, kvh, lane);
+            });
+            load_v<HD>(r, a, blk, kvh, lane);
+        }
+    };
+    if constexpr (INT4 && HD == 256) {
+        if (mine > 0) {
+            load_v<HD>(r, a, blk, kvh, lane);
+            fold_all();
+            use(mine - 1, [] {});
+        }
+    } else {
+        if (mine > 0) load_v<HD>(r, a, blk, kvh, lane);
+        fold_all();
+        if (mine > 0) use(mine - 1, [] {});
     }
-    if (mine > 0) use(mine - 1, [] {});
     const float factor = __builtin_amdgcn_exp2f(kUp - f.up);  // records have 2^kUp
     const float l = sum_x32(sum_x16(f.l)) * factor;
-    if constexpr (!INT4) {  // the low parts' rows
+    // rows 8-15 onto rows 0-7: tile 2 k's sums in the lower half of the lanes, tile
+    // 2 k + 1's in the upper
 #pragma unroll
-        for (int nt = 0; nt < HD / 16; ++nt)
+    for (int nt = 0; nt < HD / 16; nt += 2)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f.o[nt][j] = sum_x32(f.o[nt][j]);
-    }
+        for (int j = 0; j < 4; ++j) f.o[nt / 2][j] = halves_sum(f.o[nt][j], f.o[nt + 1][j]);
     // one record per wavefront in LDS: O[8][HD], M[8], L[8] (rows past H hold anything)
     constexpr int MO = kHeadsPerBlock * HD, LO = MO + kHeadsPerBlock;
     float* my = lds + wave * kRec;
-    if (g < 2) {
 #pragma unroll
-        for (int nt = 0; nt < HD / 16; ++nt)
+    for (int i = 0; i < HD / 32; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) my[(4 * g + j) * HD + 16 * nt + t] = f.o[nt][j] * factor;
-    }
+        for (int j = 0; j < 4; ++j) my[(4 * (g & 1) + j) * HD + 32 * i + 16 * (g >> 1) + t] = f.o[i][j] * factor;
     if (lane < kHeadsPerBlock) {
         // M is NaN where the length or the table is out of range
         my[MO + lane] = bad ? __builtin_nanf("") : f.m;

@@ -1,0 +1,59 @@
+"""The compact KV cache where its arithmetic and its checks have an edge:
+precision against 64 bits with next to nothing but roundings in the
+tolerance, scores and scales at the ends of their ranges, buffers that may not
+be shared, memory that is short."""
+import numpy as np
+import pytest
+
+import test_kv_compact as kvc
+from test_kv_compact import PAGE, Held, attention, call, in_order, numbers, pack, quantize, sizes, to_pages, unpack
+
+
+def one_sequence(rng, k, v, mb):
+    """int4 pools of one sequence's k and v [n][hkv][hd], their values in 64 bits, the table."""
+    table = rng.permutation(mb).astype(np.int32)[None]
+    kp, vp = pack(*quantize(to_pages([k], table, mb, np.nan)), False), pack(*quantize(to_pages([v], table, mb, np.nan)), True)
+    n, hd = k.shape[0], k.shape[2]
+    return kp, vp, in_order(unpack(kp, hd, False), table[0], n), in_order(unpack(vp, hd, True), table[0], n), table
+
+
+def attend(ctx, q, kp, vp, table, n, weights=True, int4=True):
+    """out [hq][hd] and weights [hkv][n] of one sequence, weights from 0."""
+    (hq, hd), mb = q.shape, table.shape[1]
+    hkv = kp.shape[1]
+    h = Held(ctx, q=q.astype(np.float32), kp=kp, vp=vp, table=table, lens=np.array([n], np.int32), out=np.zeros((hq, hd), np.float16),
+             w=np.zeros((hkv, mb * PAGE), np.float32))
+    f = ctx.attn_decode_paged_int4 if int4 else ctx.attn_decode_paged_f16_acc
+    f(h["q"], h["kp"], h["vp"], h["table"], h["lens"], h["out"], h["w"] if weights else 0, 1, hq, hkv, hd, mb, kp.shape[0])
+    got = h.get("out").astype(np.float64), h.get("w")[:, :n].astype(np.float64)
+    h.free()
+    return got
+
+
+# --------------------------------------------------- roundings of the products --
+@pytest.mark.gpu
+@pytest.mark.parametrize("weights", [True, False], ids=["weights", "plain"])
+@pytest.mark.parametrize("hq,hkv,hd,n", [(4, 1, 64, 31), (8, 2, 128, 60), (2, 2, 256, 500), (20, 1, 128, 1000)])
+def test_probabilities_keep_more_than_fp16(ctx, hq, hkv, hd, n, weights):
+    """Each query looks at one dimension of K alone, with a power of two there,
+    so a score is one exact product, its scale and one factor: it is off by
+    3 * 2^-24 of itself (the scale's product, the factor, its product) and e is
+    2 es + 2^-19 as elsewhere.  p * scale as fp16 hi + lo: 2^-21 of a term, or
+    half a step of the smallest numbers, 2^-25 of 2^11 and more, times a code
+    of at most 8: n 2^-33 in all.  A single fp16 number would be 2^-12 of a
+    term, which the outputs here, far smaller than their terms, do not hide."""
+    rng = np.random.default_rng(hd + n)
+    mb = -(-n // PAGE)
+    kp, vp, k64, v64, table = one_sequence(rng, rng.normal(0, 1, (n, hkv, hd)).astype(np.float32),
+                                           rng.normal(0, 1, (n, hkv, hd)).astype(np.float32), mb)
+    q = np.zeros((hq, hd))
+    q[np.arange(hq), rng.integers(0, hd, hq)] = rng.choice([-2.0, -1.0, 1.0, 2.0], hq) * 8
+    out, w = attend(ctx, q, kp, vp, table, n, weights)
+    want, W, A, _ = attention(q, k64, v64)
+    score = max(np.abs(k64[:, j] @ q[j * (hq // hkv):(j + 1) * (hq // hkv)].T).max() for j in range(hkv)) / np.sqrt(hd)
+    e = 6 * 2.0**-24 * score + 2.0**-19
+    tol = 2.0**-11 * np.abs(want) + (e + 2.0**-19) * A + n * 2.0**-33 + 2.0**-25
+    off = np.abs(out - want)
+    assert (off <= tol).all(), f"off by {(off / tol).max():.3g} of the bound"
+    if weights:
+        assert (np.abs(w - W) <= (e + 2.0**-22) * W + 2.0**-40).all()
