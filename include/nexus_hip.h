@@ -85,6 +85,15 @@ const char* nx_source_hash(void);
  * Device memory, zero-filled. */
 nx_status nx_alloc(nx_ctx* ctx, size_t bytes, nx_buf* out);
 nx_status nx_free(nx_ctx* ctx, nx_buf buf);
+/* A buffer of device memory that the caller owns (of another library, or a
+ * part of a larger allocation): `bytes` from ptr on, 16-byte aligned, inside
+ * one allocation of the context's device and outside every other buffer of
+ * the context (NX_ERR_INVALID otherwise).  Nothing is copied.  The context's
+ * stream is its own: work that fills the memory has to be complete before a
+ * call that uses it, and what calls write is there after nx_synchronize.
+ * nx_free waits for the stream and gives back the handle alone; the memory must
+ * stay until then (or until nx_destroy). */
+nx_status nx_wrap(nx_ctx* ctx, void* ptr, size_t bytes, nx_buf* out);
 /* ComputeDispatch::upload_to_gpu (compute_dispatch.h:203); replaces the UMA
  * memcpy into a shared MTLBuffer (metal_backend.mm:836-850).  Synchronous. */
 nx_status nx_upload(nx_ctx* ctx, nx_buf dst, size_t dst_offset, const void* src, size_t bytes);

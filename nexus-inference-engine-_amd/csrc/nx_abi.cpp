@@ -247,7 +247,8 @@ nx_status nx_destroy(nx_ctx* ctx) {
     for (hipGraphExec_t e : ctx->seg_exec)
         if (e) (void)hipGraphExecDestroy(e);
     if (ctx->ffn_ws) (void)hipFree(ctx->ffn_ws);
-    for (auto& kv : ctx->bufs) (void)hipFree(reinterpret_cast<void*>(kv.first));
+    for (auto& kv : ctx->bufs)
+        if (!ctx->wrapped.count(kv.first)) (void)hipFree(reinterpret_cast<void*>(kv.first));
     if (ctx->attn_ws) (void)hipFree(ctx->attn_ws);
     if (ctx->attn_counts) (void)hipFree(ctx->attn_counts);
     if (ctx->attn_chk) (void)hipFree(ctx->attn_chk);
@@ -287,7 +288,41 @@ nx_status nx_alloc(nx_ctx* ctx, size_t bytes, nx_buf* out) {
         return nx::hip_fail(ctx, e, "hipMemsetAsync");
     }
     ctx->bufs[reinterpret_cast<uint64_t>(p)] = bytes;
+    ctx->wrapped.erase(reinterpret_cast<uint64_t>(p));  // (memory given back under its handle)
     *out = reinterpret_cast<uint64_t>(p);
+    return NX_OK;
+}
+
+nx_status nx_wrap(nx_ctx* ctx, void* ptr, size_t bytes, nx_buf* out) {
+    if (!ctx || !out) return NX_ERR_INVALID;
+    const uint64_t at = reinterpret_cast<uint64_t>(ptr);
+    if (!ptr || bytes == 0 || bytes > UINT64_MAX - at) return fail(ctx, NX_ERR_INVALID, "nx_wrap: no memory (%p, %zu bytes)", ptr, bytes);
+    if (at % 16) return fail(ctx, NX_ERR_INVALID, "nx_wrap: %p is not aligned to 16 bytes", ptr);
+    if (ctx->capturing) return fail(ctx, NX_ERR_STATE, "nx_wrap inside a token batch");
+    // two handles to the same bytes would pass for two buffers where a call asks for two
+    const auto next = ctx->bufs.lower_bound(at);
+    if ((next != ctx->bufs.end() && next->first < at + bytes) ||
+        (next != ctx->bufs.begin() && std::prev(next)->first + std::prev(next)->second > at))
+        return fail(ctx, NX_ERR_INVALID, "nx_wrap: the memory is, or overlaps, a buffer of the context");
+    if (ctx->device < 0) return fail(ctx, NX_ERR_NO_DEVICE, "nx_wrap: no device");
+    hipPointerAttribute_t attr{};
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (hipPointerGetAttributes(&attr, ptr) != hipSuccess || attr.type != hipMemoryTypeDevice || attr.device != ctx->device ||
+        hipMemGetAddressRange(&base, &size, ptr) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(ctx, NX_ERR_INVALID, "nx_wrap: %p is no memory of device %d", ptr, ctx->device);
+    }
+    if (bytes > size - (at - reinterpret_cast<uint64_t>(base)))
+        return fail(ctx, NX_ERR_INVALID, "nx_wrap: %zu bytes at %p pass the end of their allocation", bytes, ptr);
+    try {
+        ctx->wrapped.insert(at);
+        ctx->bufs[at] = bytes;
+    } catch (...) {
+        ctx->wrapped.erase(at);
+        return fail(ctx, NX_ERR_OOM, "nx_wrap: no memory for the handle");
+    }
+    *out = at;
     return NX_OK;
 }
 
@@ -297,7 +332,7 @@ nx_status nx_free(nx_ctx* ctx, nx_buf b) {
     auto it = ctx->bufs.find(b);
     if (it == ctx->bufs.end()) return fail(ctx, NX_ERR_INVALID, "nx_free: unknown buffer");
     NX_HIP(ctx, hipStreamSynchronize(ctx->stream));
-    NX_HIP(ctx, hipFree(reinterpret_cast<void*>(b)));
+    if (!ctx->wrapped.erase(b)) NX_HIP(ctx, hipFree(reinterpret_cast<void*>(b)));
     ctx->bufs.erase(it);
     for (auto w = ctx->wcache.begin(); w != ctx->wcache.end();)
         w = (w->second == b) ? ctx->wcache.erase(w) : std::next(w);

@@ -6,6 +6,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <map>
+#include <set>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -16,6 +17,7 @@ struct nx_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
     std::map<uint64_t, size_t> bufs;                   // device address -> bytes
+    std::set<uint64_t> wrapped;                        // those of bufs whose memory is the caller's
     std::unordered_map<const void*, uint64_t> wcache;  // host key -> buffer
     std::string err;
     bool capturing = false;

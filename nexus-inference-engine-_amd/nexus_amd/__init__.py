@@ -95,6 +95,7 @@ _SIGS = {
     "nx_source_hash": (C.c_char_p, []),
     "nx_alloc": (_I, [_P, C.c_size_t, C.POINTER(_B)]),
     "nx_free": (_I, [_P, _B]),
+    "nx_wrap": (_I, [_P, _P, C.c_size_t, C.POINTER(_B)]),
     "nx_upload": (_I, [_P, _B, C.c_size_t, _P, C.c_size_t]),
     "nx_download": (_I, [_P, _P, _B, C.c_size_t, C.c_size_t]),
     "nx_weight_cache": (_I, [_P, _P, _P, C.c_size_t, C.POINTER(_B)]),
@@ -297,6 +298,16 @@ class Context:
     def alloc(self, nbytes: int) -> int:
         b = C.c_uint64()
         self.check(self.L.nx_alloc(self.h, int(nbytes), C.byref(b)), "nx_alloc")
+        return b.value
+
+    def wrap(self, ptr: int, nbytes: int) -> int:
+        """A buffer of device memory that the caller owns (a torch tensor's
+        data_ptr(), say).  The context's stream is its own: what fills the
+        memory has to be complete before a call uses it, and what calls write
+        is there after sync().  free() gives back the handle, and the memory
+        must stay until then."""
+        b = C.c_uint64()
+        self.check(self.L.nx_wrap(self.h, int(ptr), int(nbytes), C.byref(b)), "nx_wrap")
         return b.value
 
     def free(self, b: int):
