@@ -185,7 +185,7 @@ def _inputs(case, seed):
     return t
 
 
-# -------------------------------------------------- the library and its buffers --
+# -------------------------------------------------- the library and its handles --
 _CTX = None
 
 
@@ -201,45 +201,35 @@ def _context():
     return _CTX
 
 
-class Buffer:
-    """A library buffer given back with its last user; t is a torch view of it."""
+class State:
+    """A case's tensors and, for the library, its handles to them, which end
+    before the tensors do (free waits for the calls that use them)."""
 
-    _TYPES = {torch.float32: "<f4", torch.float16: "<f2", torch.uint8: "|u1", torch.int32: "<i4"}
-
-    def __init__(self, value):
-        self.ctx = _context()
-        self.id = self.ctx.alloc(value.numel() * value.element_size())
-        self.ctx.sync()
-        self.__cuda_array_interface__ = dict(shape=tuple(value.shape), typestr=self._TYPES[value.dtype],
-                                             data=(self.id, False), version=2)
-        self.t.copy_(value)
-        torch.cuda.synchronize()
-
-    @property
-    def t(self):
-        return torch.as_tensor(self, device="cuda")  # holds a reference to this buffer
+    def __init__(self, case, tensors):
+        self.case, self.t, self.id = case, tensors, {}
 
     def __del__(self):
         try:
-            self.ctx.free(self.id)
+            for b in self.id.values():
+                self.ctx.free(b)
         except Exception:
             pass
 
 
-class State:
-    pass
-
-
 def prepare(case, seed):
-    s = State()
-    s.case, s.t = case, _inputs(case, seed)
-    if own:  # the library works on its own buffers, which a program holds by handle
-        held = {n: Buffer(v) for n, v in s.t.items()}
-        s.ctx, s.id, s.t = _context(), {n: b.id for n, b in held.items()}, {n: b.t for n, b in held.items()}
+    s = State(case, _inputs(case, seed))
+    if own:  # the library works on the tensors' own memory
+        s.ctx = _context()
+        for n, v in s.t.items():
+            s.id[n] = s.ctx.wrap(v.data_ptr(), v.numel() * v.element_size())
+        torch.cuda.synchronize()  # its stream is its own: the inputs have to be there
     return s
 
 
 # -------------------------------------------------------- the library's calls --
+# Queued on the context's stream, which torch's know nothing of: a program that
+# goes on to read the outputs calls the context's sync() first, and one that
+# queues more calls does not.
 def _run_own(s):
     c, i, t, ctx = s.case, s.id, s.t, s.ctx
     B, hkv, hd, mb = c["batch"], c["hkv"], c["hd"], _max_blocks(c)
