@@ -298,9 +298,10 @@ nx_status nx_attn_decode_paged_f16_acc(nx_ctx* ctx, nx_buf q_f32, nx_buf kpool, 
  * are then [0, keep) in no particular order, which attention does not mind
  * (keys carry their rotation).  weights_out and tags_out get the slots' weights
  * and tags, zeros from the new length on; lens_out[b] the new length, the next
- * token's slot; pages past it are free.  Each of the three may be its input.  A
- * sequence of at most `keep` tokens moves nothing.  One whose length is out of
- * range or above seen[b], or whose table names a block outside the pool, gets
+ * token's slot; pages past it are free.  Each of the three may be its input; the
+ * pools and the three are no other buffer of the call otherwise.  A sequence
+ * of at most `keep` tokens moves nothing.  One whose length is out of range or
+ * above seen[b], or whose table names a block outside the pool, gets
  * lens_out[b] = -1 and stays as it is.  No page may belong to two sequences, or
  * twice to one. */
 nx_status nx_kv_evict_f16(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block_table, nx_buf ctx_lens_i32, nx_buf seen_i32,

@@ -178,11 +178,14 @@ nx_status evict(nx_ctx* ctx, const char* name, bool int4, nx_buf kpool, nx_buf v
     NX_NEED(ctx, lens_out, (size_t)batch * 4, "lens_out");
     NX_NEED(ctx, w_out, slots, "weights_out");
     NX_NEED(ctx, t_out, slots, "tags_out");
-    // an output may be the input of its kind and no other buffer of the call
-    const nx_buf in[] = {kpool, vpool, bt, lens_in, seen, w_in, t_in}, outs[] = {lens_out, w_out, t_out}, own[] = {lens_in, w_in, t_in};
-    bool clash = kpool == vpool || lens_out == w_out || lens_out == t_out || w_out == t_out;
-    for (int i = 0; i < 3; ++i)
-        for (nx_buf b : in) clash = clash || (outs[i] == b && b != own[i]);
+    // What is written is no other buffer of the call, but that each of the last
+    // three may be the input of its kind.  (The places count: an input that is
+    // given twice may not be one output's own and stand for another input.)
+    const nx_buf all[] = {kpool, vpool, lens_out, w_out, t_out, bt, seen, lens_in, w_in, t_in};
+    constexpr int kWritten = 5, kAll = 10;
+    bool clash = false;
+    for (int i = 0; i < kWritten; ++i)
+        for (int j = 0; j < kAll; ++j) clash = clash || (j != i && all[j] == all[i] && !(i >= 2 && j == i + 5));
     if (clash) return fail(ctx, NX_ERR_INVALID, "%s: an output is another buffer of the call", name);
     if (ctx->device < 0) return fail(ctx, NX_ERR_NO_DEVICE, "%s: no device", name);
     const OnDevice on(ctx->device);

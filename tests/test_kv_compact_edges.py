@@ -57,3 +57,25 @@ def test_probabilities_keep_more_than_fp16(ctx, hq, hkv, hd, n, weights):
     assert (off <= tol).all(), f"off by {(off / tol).max():.3g} of the bound"
     if weights:
         assert (np.abs(w - W) <= (e + 2.0**-22) * W + 2.0**-40).all()
+
+
+# ------------------------------------------------------------ shared buffers --
+@pytest.mark.parametrize("op", ["nx_kv_evict_f16", "nx_kv_evict_int4"])
+def test_eviction_refuses_pools_that_are_another_buffer(op):
+    """Both pools are written: neither may be the table, whose checked entries
+    the moves go by, nor any other buffer of the call."""
+    n = len(sizes(op, kvc.SHAPE))
+    ids, big = list(range(1, n + 1)), [1 << 20] * n
+    assert call(op, ids, kvc.SHAPE, big)[0] == 6
+    for pool in (0, 1):
+        for i in range(n):
+            if i != pool:
+                st, msg = call(op, ids[:pool] + [ids[i]] + ids[pool + 1:], kvc.SHAPE, big)
+                assert st == 1 and "another buffer" in msg, (pool, i)
+    # outputs in place of inputs that are given twice: the other input would change under the call
+    for same, out in (((4, 3), 7), ((6, 5), 8), ((5, 6), 9)):
+        twice = list(ids)
+        twice[same[0]] = twice[same[1]]
+        assert call(op, twice, kvc.SHAPE, big)[0] == 6  # (read alone, that is no harm)
+        twice[out] = twice[same[1]]
+        assert call(op, twice, kvc.SHAPE, big)[0] == 1, out
