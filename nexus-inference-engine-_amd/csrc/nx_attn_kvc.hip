@@ -262,10 +262,11 @@ struct Fold {
 
 // ------------------------------------------------------------ values of a pair --
 // The powers of two that a pair's probabilities may have.  P V takes p
-// times the token's scale as fp16 numbers (below).  With p up to 2^15 a
-// scale of 2 or more (a value of 16 and up among a group) could pass the
-// largest fp16 number: from such a pair on the wavefront's factor is as many
-// powers of two smaller.
+// times the token's scale as fp16 numbers (below).  p is 2^15 at most, and as
+// much more as the roundings of scores below kFar give (2^-4 in the exponent
+// at 2^20), so with a scale of 1 or more (a value of 8 and up among a group) the
+// product could pass the largest fp16 number: from such a pair on the
+// wavefront's factor is as many powers of two smaller, down to 2^-5.
 template <int HD>
 __device__ inline float most_up(const PairI4<HD>& r, float up) {
     typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
@@ -279,7 +280,7 @@ __device__ inline float most_up(const PairI4<HD>& r, float up) {
             most = __builtin_elementwise_max(most, __builtin_elementwise_max(__builtin_shufflevector(w, w, 0, 1), __builtin_shufflevector(w, w, 2, 3)));
         }
     const int e = max((int)most.x, (int)most.y) >> 10;  // biased exponent: 15 is 2^0
-    constexpr int kTop = 15 + (int)kUp;
+    constexpr int kTop = 14 + (int)kUp;
     return __any(e > kTop - (int)up) ? (float)kTop - wave_max((float)e) : up;
 }
 template <int HD>

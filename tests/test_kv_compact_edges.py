@@ -59,6 +59,38 @@ def test_probabilities_keep_more_than_fp16(ctx, hq, hkv, hd, n, weights):
         assert (np.abs(w - W) <= (e + 2.0**-22) * W + 2.0**-40).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("big,first,code,second,score", [
+    (224.875, 1.669921875, 1, 3.408203125, 18168), (1614.0, 1.1396484375, 3, 3.6640625, 130397),
+    (6976.0, 2.4296875, 6, 5.23828125, 563600)])
+def test_largest_probability_times_largest_scale(ctx, big, first, code, second, score):
+    """Scores far from 0 (`score`, times log2 e) whose maximum moves by 4 in log2
+    and, by the roundings of fp32 there, up to 2^-5 more than a wavefront can see:
+    it keeps its reference, and a probability passes 2^15.  With a scale of
+    nearly 2 the product passes 65504, fp16's largest number, though every input is far
+    from any limit.  All tokens have the same V, so that is the output, whatever
+    the weights: the sum of p times V over the sum of p, 2^-19 off, and rounded.  A
+    weight comes from its score, rounded, and from L, whose references are: 3
+    roundings of numbers of about `score` in an exponent."""
+    rng = np.random.default_rng(score)
+    hd, n = 64, 512 * 2 * PAGE  # pairs of pages 0..255 hold the first maximum, the others the second
+    k, v = np.zeros((n, 1, hd), np.float32), np.zeros((n, 1, hd), np.float32)
+    at = np.arange(512) * 2 * PAGE + rng.integers(0, 2 * PAGE, 512)
+    k[at, 0, 0] = 7 * big
+    k[at[:256], 0, 32], k[at[:256], 0, 33] = code * first, 7 * first
+    k[at[256:], 0, 32] = 7 * second
+    v[:, 0] = rng.integers(-7, 8, hd) * np.float32(1.9990234375)
+    v[:, 0, 5] = v[:, 0, 40] = 7 * 1.9990234375
+    q = np.zeros((1, hd))
+    q[0, 0], q[0, 32] = 64, 1
+    kp, vp, k64, v64, table = one_sequence(rng, k, v, n // PAGE)
+    assert np.array_equal(k64, k) and np.array_equal(v64, v)
+    assert abs((k64[at[0], 0] @ q[0]) / 8 * np.log2(np.e) - score) < 1
+    out, w = attend(ctx, q, kp, vp, table, n)
+    assert (np.abs(out[0] - v[0, 0]) <= (2.0**-11 + 2.0**-19) * np.abs(v[0, 0])).all()
+    assert abs(w.sum() - 1) <= 3 * 2.0**-24 * score * np.log(2) + 2.0**-19
+
+
 # ------------------------------------------------------------ shared buffers --
 @pytest.mark.parametrize("op", ["nx_kv_evict_f16", "nx_kv_evict_int4"])
 def test_eviction_refuses_pools_that_are_another_buffer(op):
