@@ -266,22 +266,27 @@ struct Fold {
 // much more as the roundings of scores below kFar give (2^-4 in the exponent
 // at 2^20), so with a scale of 1 or more (a value of 8 and up among a group) the
 // product could pass the largest fp16 number: from such a pair on the
-// wavefront's factor is as many powers of two smaller, down to 2^-5.
+// wavefront's factor is as many powers of two smaller, down to 2^-5.  (What fp16's
+// smallest number, 2^-24, then leaves out of a token's term is 2^-34 of the largest
+// |V| among the wavefront's tokens.)
 template <int HD>
 __device__ inline float most_up(const PairI4<HD>& r, float up) {
     typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
     typedef uint16_t us4_t __attribute__((ext_vector_type(4)));
-    us2_t most = {0, 0};
+    auto most = [&](uint16_t bits) {  // of the scales, each masked
+        us2_t m = {0, 0};
 #pragma unroll
-    for (int pg = 0; pg < 2; ++pg)
+        for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-            const us4_t w = __builtin_bit_cast(us4_t, r.vs[pg][i]);
-            most = __builtin_elementwise_max(most, __builtin_elementwise_max(__builtin_shufflevector(w, w, 0, 1), __builtin_shufflevector(w, w, 2, 3)));
-        }
-    const int e = max((int)most.x, (int)most.y) >> 10;  // biased exponent: 15 is 2^0
+            for (int i = 0; i < HD / 32; ++i) {
+                const us4_t w = __builtin_bit_cast(us4_t, r.vs[pg][i]) & bits;
+                m = __builtin_elementwise_max(m, __builtin_elementwise_max(__builtin_shufflevector(w, w, 0, 1), __builtin_shufflevector(w, w, 2, 3)));
+            }
+        return max((int)m.x, (int)m.y) >> 10;  // biased exponent: 15 is 2^0 (and 32 and up: a negative one)
+    };
     constexpr int kTop = 14 + (int)kUp;
-    return __any(e > kTop - (int)up) ? (float)kTop - wave_max((float)e) : up;
+    if (!__any(most(0xFFFFu) > kTop - (int)up)) return up;
+    return fminf(up, (float)kTop - wave_max((float)most(0x7FFFu)));
 }
 template <int HD>
 __device__ inline float most_up(const PairF16<HD>&, float up) {

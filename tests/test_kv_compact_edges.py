@@ -91,6 +91,34 @@ def test_largest_probability_times_largest_scale(ctx, big, first, code, second, 
     assert abs(w.sum() - 1) <= 3 * 2.0**-24 * score * np.log(2) + 2.0**-19
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,n", [(64, 31), (128, 600), (256, 90)])
+def test_scales_of_either_sign(ctx, hd, n):
+    """The format's value is (code - 8) * scale: negated scales with negated
+    codes are the same values, and give the same outputs (the tolerance of
+    test_probabilities_keep_more_than_fp16)."""
+    rng = np.random.default_rng(hd * n)
+    mb = -(-n // PAGE)
+    table = rng.permutation(mb).astype(np.int32)[None]
+    pools, vals = [], []
+    for value in (False, True):
+        codes, s = quantize(to_pages([rng.normal(0, 1, (n, 1, hd)).astype(np.float32)], table, mb, 0))
+        codes = np.maximum(codes, 1)  # (code 0 has no negative)
+        flip = rng.random(s.shape) < 0.5
+        codes = np.where(np.repeat(flip, 32, -1), 16 - codes, codes).astype(np.uint8)
+        pools.append(pack(codes, np.where(flip, -s, s).astype(np.float16), value))
+        vals.append(in_order(unpack(pools[-1], hd, value), table[0], n))
+    q = np.zeros((3, hd))
+    q[np.arange(3), [3, hd // 2, hd - 1]] = [16, -8, 8]
+    out, w = attend(ctx, q, *pools, table, n)
+    want, W, A, _ = attention(q, *vals)
+    e = 6 * 2.0**-24 * np.abs(vals[0][:, 0] @ q.T).max() / np.sqrt(hd) + 2.0**-19
+    tol = 2.0**-11 * np.abs(want) + (e + 2.0**-19) * A + n * 2.0**-33 + 2.0**-25
+    off = np.abs(out - want)
+    assert (off <= tol).all(), f"off by {(off / tol).max():.3g} of the bound"
+    assert (np.abs(w - W) <= (e + 2.0**-22) * W + 2.0**-40).all()
+
+
 # ------------------------------------------------------------ shared buffers --
 @pytest.mark.parametrize("op", ["nx_kv_evict_f16", "nx_kv_evict_int4"])
 def test_eviction_refuses_pools_that_are_another_buffer(op):
