@@ -274,9 +274,9 @@ nx_status nx_kv_read_int4(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block_
  * length exceeds max_blocks * 16 (or is negative), or whose table names a block
  * outside [0, num_blocks) for one of its pages, gets NaN output rows and its
  * weights stay as they are.  A cached value of its positions that is not
- * finite makes outputs NaN or infinite (K: its kv head's, and the weights; V:
- * its dimension's, of int4 pages its group's); slots past the length may hold
- * anything.  No output or weights buffer may be another buffer of the call. */
+ * finite shows: K's makes its kv head's rows and weights NaN, V's makes its
+ * dimension (of int4 pages its group) NaN or infinite; one of q makes its head's
+ * row and the kv head's weights NaN.  Slots past the length may hold anything.  No output or weights buffer may be another buffer of the call. */
 nx_status nx_attn_decode_paged_int4(nx_ctx* ctx, nx_buf q_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
                                     nx_buf ctx_lens_i32, nx_buf out_f16, nx_buf weights_f32, int batch, int hq, int hkv,
                                     int head_dim, int max_blocks, int num_blocks);

@@ -409,7 +409,12 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, const f4_t* off
     next_k();
     float p[8], top = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = s[j / 4][j % 4] + dpp<kRowRor8>(s[j / 4][j % 4]);
+    for (int j = 0; j < 8; ++j) {
+        p[j] = s[j / 4][j % 4] + dpp<kRowRor8>(s[j / 4][j % 4]);
+        // An infinite key gives infinities and NaN by the signs of q's two parts:
+        // NaN for any.  (No finite one passes fp32 here.)
+        p[j] = __builtin_fmaf(p[j], 0.0f, p[j]);
+    }
     if (nb < kPage) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[j] = 4 * g + j % 4 < (j < 4 ? na : nb) ? p[j] : -__builtin_inff();

@@ -119,6 +119,43 @@ def test_scales_of_either_sign(ctx, hd, n):
     assert (np.abs(w - W) <= (e + 2.0**-22) * W + 2.0**-40).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+def test_an_infinite_key_of_fp16_pages(ctx, hd, value):
+    """Whatever the signs of q and of its rounding to fp16, and whether that
+    leaves a rest: an infinite element of K makes every row and weight of its
+    kv head NaN, and no other head's."""
+    rng = np.random.default_rng(hd)
+    hq, hkv, n, mb = 16, 2, 50, 4
+    table = np.arange(mb, dtype=np.int32)[None]
+    k, v = rng.normal(0, 1, (2, n, hkv, hd)).astype(np.float32)
+    k[20, 0, 5] = value
+    kp, vp = to_pages([k], table, mb, 0).astype(np.float16), to_pages([v], table, mb, 0).astype(np.float16).transpose(0, 1, 3, 2)
+    q = rng.normal(0, 1, (hq, hd))
+    # of the first kv head's eight: either sign, a rest of either sign and none
+    q[:8, 5] = [1, -1, 1 + 2.0**-13, 1 - 2.0**-13, -1 - 2.0**-13, -1 + 2.0**-13, 2, 1e-3]
+    out, w = attend(ctx, q, kp, vp, table, n, int4=False)
+    assert np.isnan(out[:8]).all() and np.isnan(w[0]).all()
+    assert np.isfinite(out[8:]).all() and abs(w[1].sum() - 8) < 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+def test_an_infinite_scale_of_int4_pages(ctx, hd, value):
+    """The same for pages that some other program wrote with an infinite scale."""
+    rng = np.random.default_rng(hd)
+    n, mb = 50, 4
+    table = np.arange(mb, dtype=np.int32)[None]
+    k, v = rng.normal(0, 1, (2, n, 2, hd)).astype(np.float32)
+    codes, s = quantize(to_pages([k], table, mb, 0))
+    s[1, 0, 4, 1] = value  # token 20's second group
+    out, w = attend(ctx, rng.normal(0, 1, (16, hd)), pack(codes, s, False), pack(*quantize(to_pages([v], table, mb, 0)), True), table, n)
+    assert np.isnan(out[:8]).all() and np.isnan(w[0]).all()
+    assert np.isfinite(out[8:]).all() and abs(w[1].sum() - 8) < 1e-4
+
+
 # ------------------------------------------------------------ shared buffers --
 @pytest.mark.parametrize("op", ["nx_kv_evict_f16", "nx_kv_evict_int4"])
 def test_eviction_refuses_pools_that_are_another_buffer(op):
