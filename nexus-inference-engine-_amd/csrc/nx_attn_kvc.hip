@@ -432,17 +432,17 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, const f4_t* off
     // Far from 0 (kFar) a step of the scores' 24 bits is near the powers of two
     // that p has to spare: there they are rounded and taken from the maximum
     // itself before anything is added.
-    const bool far = __any(fabsf(top) > kFar);
+    const bool far = fabsf(top) > kFar && top != -__builtin_inff();  // (of a column: heads go by their own scores)
     const float mn = top > (far ? f.m : f.m + kLead) ? top : f.m;
     const bool none = mn == -__builtin_inff();  // no token, or NaN scores alone
     const float up = most_up<HD>(r, f.up);
     const float corr = none ? 1.0f : __builtin_amdgcn_exp2f(f.m - mn + (up - f.up));
     float by = scale, from = none ? 0.0f : mn - up, sum = 0.0f;
-    if (far) {
+    if (__any(far)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = p[j] * scale - (none ? 0.0f : mn);
-        by = 1.0f;
-        from = none ? 0.0f : -up;
+        for (int j = 0; j < 8; ++j) p[j] = far ? p[j] * scale - mn : p[j];
+        by = far ? 1.0f : by;
+        from = far ? -up : from;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

@@ -141,6 +141,27 @@ def test_an_infinite_key_of_fp16_pages(ctx, hd, value):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("int4", [True, False], ids=["int4", "f16"])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan, 1e9])
+def test_a_query_far_from_the_others(ctx, int4, value):
+    """One that is not finite: its row and its kv head's weights are NaN, the other heads' rows are
+    theirs, bit for bit: what a head computes goes by its own scores."""
+    rng = np.random.default_rng(1)
+    hq, hkv, hd, n, mb = 12, 2, 64, 50, 4
+    table = np.arange(mb, dtype=np.int32)[None]
+    pk, pv = (to_pages([rng.normal(0, 1, (n, hkv, hd)).astype(np.float32)], table, mb, 0) for _ in range(2))
+    kp, vp = (pack(*quantize(pk), False), pack(*quantize(pv), True)) if int4 else (pk.astype(np.float16), pv.astype(np.float16).transpose(0, 1, 3, 2))
+    q = rng.normal(0, 1, (hq, hd))
+    want, _ = attend(ctx, q, kp, vp, table, n, int4=int4)
+    q[2, 7] = value
+    out, w = attend(ctx, q, kp, vp, table, n, int4=int4)
+    if not np.isfinite(value):
+        assert np.isnan(out[2]).all() and np.isnan(w[0]).all()
+    assert np.isfinite(w[1]).all()
+    assert np.array_equal(np.delete(out, 2, 0), np.delete(want, 2, 0))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("value", [np.inf, -np.inf])
 def test_an_infinite_scale_of_int4_pages(ctx, hd, value):
