@@ -313,6 +313,12 @@ nx_status nx_kv_evict_int4(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block
                            nx_buf weights_f32, nx_buf tags_i32, nx_buf lens_out_i32, nx_buf weights_out_f32,
                            nx_buf tags_out_i32, int batch, int hkv, int head_dim, int max_blocks, int num_blocks, int keep,
                            int recent);
+/* Grow the workspace of the attention calls and evictions above (records,
+ * scores and eviction lists: 4 bytes a sequence, query head and position, and
+ * more) to what any of them needs with at most these sizes and max_blocks up to
+ * ceil(max_ctx / 16), so that they allocate nothing and wait for nothing.
+ * Without it the first call of each larger size grows it. */
+nx_status nx_reserve_kv_compact(nx_ctx* ctx, int batch, int n_heads, int n_kv_heads, int head_dim, int max_ctx);
 /* MoE routing: softmax over E logits fp32 [batch][E], top-k by probability
  * (ties: lower id), renormalized weights.  hybrid_model.cpp:1656-1694.
  * E <= 256, k <= min(16, E), batch <= 64. */
@@ -397,10 +403,10 @@ nx_status nx_init_kv_cache(nx_ctx* ctx, int num_layers, int max_seq, int n_kv_he
  * workspace the entry points keep per context -- FFN activations, K-part
  * sums (of the down projection, and of GEMMs over a layer's matrices with up
  * to 2048 rows), sampler rows, attention split records, counters and table
- * checks, the compact cache's records, scores and eviction lists (4 bytes a
- * query head and position, and more) -- to what calls up to these sizes need, so those calls allocate
+ * checks -- to what calls up to these sizes need, so those calls allocate
  * nothing (and may be captured, where they can be at all).  A size of 0 skips its workspace.  The reference reserves staging bytes; this
- * library takes the shapes the bytes come from. */
+ * library takes the shapes the bytes come from.  (The compact cache's workspace
+ * is nx_reserve_kv_compact's.) */
 nx_status nx_reserve_workspace(nx_ctx* ctx, int batch, int max_ffn, int vocab, int n_heads, int n_kv_heads,
                                int head_dim, int max_ctx);
 /* ComputeDispatch::preload_all_buffers (compute_dispatch.h:285,

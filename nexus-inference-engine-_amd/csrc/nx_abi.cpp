@@ -1355,7 +1355,6 @@ nx_status nx_reserve_workspace(nx_ctx* ctx, int batch, int max_ffn, int vocab, i
         if (max_ctx > nx::attn_max_ctx()) return fail(ctx, NX_ERR_UNSUPPORTED, "max_ctx above the attention limit");
         s = ensure_attn_ws(ctx, nx::attn_workspace_bytes(batch, n_heads, n_kv_heads, head_dim, max_ctx));
         if (s == NX_OK) s = ensure_attn_counts(ctx, nx::attn_count_words(batch, n_kv_heads));
-        if (s == NX_OK) s = nx::kvc_reserve(ctx, batch, n_heads, n_kv_heads, head_dim, max_ctx);
         chk = nx::attn_check_words(batch, (max_ctx + nx::kPage - 1) / nx::kPage);
     }
     if (s == NX_OK) s = ensure_attn_chk(ctx, chk);  // (the routed experts' plan check as well)

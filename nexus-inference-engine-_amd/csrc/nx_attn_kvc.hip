@@ -779,10 +779,17 @@ AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4
 }
 
 size_t attn_part_floats(const AttnPlan& p, int batch, int hkv) { return (size_t)batch * hkv * p.groups * p.splits * p.rec; }
-size_t attn_most_part_floats(int batch, int hq, int hkv, int hd) {
-    AttnPlan p = heads_plan(hq, hkv, hd);
-    p.splits = kMaxSplits;
-    return attn_part_floats(p, batch, hkv);
+// (Records grow with the heads that share a kv head but for steps of eight, so
+// fewer kv heads can take more: each number with the most heads for it.  A call of
+// fewer rows may split its pages further: up to the most splits.)
+size_t attn_most_part_floats(int batch, int hq, int hkv, int hd, int max_blocks, int max_group) {
+    size_t most = 0;
+    for (int h = 1; h <= std::min(hq, hkv); ++h) {
+        AttnPlan p = heads_plan(std::min(hq / h, max_group) * h, h, hd);
+        p.splits = std::min(kMaxSplits, (max_blocks + 1) / 2);
+        most = std::max(most, attn_part_floats(p, batch, h));
+    }
+    return most;
 }
 
 hipError_t attn_launch(const AttnArgs& a, bool int4, hipStream_t st) {

@@ -98,9 +98,6 @@ hipError_t dev_malloc(nx_ctx* ctx, T** p, size_t bytes) {
     return dev_malloc(ctx, reinterpret_cast<void**>(p), bytes);
 }
 
-// The compact cache's part of nx_reserve_workspace.
-nx_status kvc_reserve(nx_ctx* ctx, int batch, int hq, int hkv, int hd, int max_ctx);
-
 // Size of a buffer of the context, 0 if it is not one.
 inline size_t buf_size(const nx_ctx* ctx, nx_buf b) {
     auto it = ctx->bufs.find(b);

@@ -216,17 +216,6 @@ nx_status evict(nx_ctx* ctx, const char* name, bool int4, nx_buf kpool, nx_buf v
 
 }  // namespace
 
-namespace nx {
-nx_status kvc_reserve(nx_ctx* ctx, int batch, int hq, int hkv, int hd, int max_ctx) {
-    if (hd != 64 && hd != 128 && hd != 256) return NX_OK;
-    const int blocks = (max_ctx + kPage - 1) / kPage;
-    // (a call of less may split its pages further: records for the most splits)
-    const size_t attn = 4 * (kvc::attn_most_part_floats(batch, hq, hkv, hd) + kvc::attn_raw_floats(batch, hq, blocks));
-    const size_t bytes = std::max(4 * kvc::evict_ws_words(batch, hkv, blocks, blocks * kPage), attn);
-    return kvc_ws(ctx, bytes, "nx_reserve_workspace");
-}
-}  // namespace nx
-
 extern "C" {
 
 // Not part of the interface: the pages that the row kernels work on, for a
@@ -238,6 +227,20 @@ int nx_kvc_row_page(int first, int tokens, int max_blocks, int i, int* out) {
     out[2] = p.none;
     out[3] = p.refused;
     return nx::kvc::row_pages(tokens);
+}
+
+nx_status nx_reserve_kv_compact(nx_ctx* ctx, int batch, int hq, int hkv, int hd, int max_ctx) {
+    const char* name = "nx_reserve_kv_compact";
+    if (!ctx) return NX_ERR_INVALID;
+    if (hq < 1 || max_ctx < 1) return fail(ctx, NX_ERR_INVALID, "%s: bad sizes (n_heads=%d max_ctx=%d)", name, hq, max_ctx);
+    const int blocks = (int)(((int64_t)max_ctx + nx::kPage - 1) / nx::kPage);
+    const nx_status s = cache_shape(ctx, name, batch, hkv, hd, blocks, 1);
+    if (s != NX_OK) return s;
+    if (ctx->capturing) return fail(ctx, NX_ERR_STATE, "%s inside a token batch", name);
+    if (ctx->device < 0) return fail(ctx, NX_ERR_NO_DEVICE, "%s: no device", name);
+    const OnDevice on(ctx->device);
+    const size_t attn = 4 * (nx::kvc::attn_most_part_floats(batch, hq, hkv, hd, blocks, kMaxGroup) + nx::kvc::attn_raw_floats(batch, hq, blocks));
+    return kvc_ws(ctx, std::max(4 * nx::kvc::evict_ws_words(batch, hkv, blocks, blocks * nx::kPage), attn), name);
 }
 
 nx_status nx_kv_append_int4(nx_ctx* ctx, nx_buf k, nx_buf v, nx_buf kpool, nx_buf vpool, nx_buf bt, nx_buf pos, int batch, int tokens, int hkv,

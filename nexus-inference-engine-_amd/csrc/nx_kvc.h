@@ -80,7 +80,7 @@ struct AttnArgs {
 };
 // Floats of the workspace: the records, and the scores with weights.
 size_t attn_part_floats(const AttnPlan& p, int batch, int hkv);
-size_t attn_most_part_floats(int batch, int hq, int hkv, int hd);  // of any plan up to these sizes
+size_t attn_most_part_floats(int batch, int hq, int hkv, int hd, int max_blocks, int max_group);  // of any call up to these sizes
 inline size_t attn_raw_floats(int batch, int hq, int max_blocks) { return (size_t)batch * hq * max_blocks * kPage; }
 hipError_t attn_launch(const AttnArgs& a, bool int4, hipStream_t st);
 

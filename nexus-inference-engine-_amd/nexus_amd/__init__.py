@@ -133,6 +133,7 @@ _SIGS = {
     "nx_attn_decode_paged_f16_acc": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I]),
     "nx_kv_evict_f16": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I, _I]),
     "nx_kv_evict_int4": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I, _I, _I, _I]),
+    "nx_reserve_kv_compact": (_I, [_P, _I, _I, _I, _I, _I]),
     "nx_tq_codebooks": (_I, [_P, _P, _P, _P]),
     "nx_tq_encode": (_I, [_P, _B, _B, _B, _B, _B, _I]),
     "nx_tq_append": (_I, [_P, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _B, _I, _I, _I, _I]),
@@ -343,6 +344,9 @@ class Context:
                    "nx_gemv_int4_g32_f32")
 
     # the compact KV cache (include/nexus_hip.h); buffers are handles
+    def reserve_kv_compact(self, batch, hq, hkv, head_dim, max_ctx):
+        self.check(self.L.nx_reserve_kv_compact(self.h, batch, hq, hkv, head_dim, max_ctx), "nx_reserve_kv_compact")
+
     def kv_append_int4(self, k, v, kpool, vpool, table, positions, batch, tokens, hkv, head_dim, max_blocks, num_blocks):
         self.check(self.L.nx_kv_append_int4(self.h, k, v, kpool, vpool, table, positions, batch, tokens, hkv, head_dim,
                                             max_blocks, num_blocks), "nx_kv_append_int4")

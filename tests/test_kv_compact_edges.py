@@ -197,3 +197,59 @@ def test_eviction_refuses_pools_that_are_another_buffer(op):
         assert call(op, twice, kvc.SHAPE, big)[0] == 6  # (read alone, that is no harm)
         twice[out] = twice[same[1]]
         assert call(op, twice, kvc.SHAPE, big)[0] == 1, out
+
+
+# ---------------------------------------------------------------- workspaces --
+def test_reserve_refusals():
+    L = kvc.nexus_amd.lib()
+    L.nx_deviceless.restype = kvc.C.c_void_p
+    ctx = kvc.C.c_void_p(L.nx_deviceless((kvc.C.c_size_t * 1)(1), 1))
+    good = (2, 16, 4, 128, 2048)
+    assert L.nx_reserve_kv_compact(ctx, *good) == 6
+    assert L.nx_reserve_kv_compact(None, *good) == 1
+    for i in range(5):
+        for bad in (0, -1):
+            assert L.nx_reserve_kv_compact(ctx, *good[:i], bad, *good[i + 1:]) == 1, i
+    for bad in ((65536, 16, 4, 128, 2048), (2, 8194, 4097, 128, 2048), (2, 16, 4, 32, 2048), (2, 16, 4, 128, (1 << 26) + 1)):
+        assert L.nx_reserve_kv_compact(ctx, *bad) == 4, bad
+    L.nx_destroy(ctx)
+
+
+@pytest.mark.gpu
+def test_reserving_for_the_other_calls_takes_no_more_than_they_need(poor):
+    """8 sequences of 32 heads and 131072 positions, in allocations of 64 MiB at
+    most: the split records of attention are a few MiB.  (The scores of the
+    calls that accumulate weights would be 128 MiB.)"""
+    poor.limit(64 << 20)
+    poor.check(poor.L.nx_reserve_workspace(poor.h, 8, 0, 0, 32, 8, 128, 131072), "reserve")
+
+
+@pytest.mark.gpu
+def test_reserved_calls_allocate_nothing(poor):
+    """After nx_reserve_kv_compact every later allocation may fail: calls of
+    fewer sequences, heads, kv heads, dimensions or positions run, whichever are fewer."""
+    poor.check(poor.L.nx_reserve_kv_compact(poor.h, 3, 18, 18, 128, 2000), "reserve")
+    rng = np.random.default_rng(3)
+    cases = []
+    for hq, hkv, hd, lens in ((18, 18, 128, [2000, 5, 700]), (18, 1, 128, [1999] * 3), (18, 2, 64, [40]), (9, 1, 128, [2000, 1]), (18, 6, 64, [2000] * 3)):
+        for int4 in (True, False):
+            B, mb = len(lens), -(-max(lens) // PAGE)
+            kp, vp, k64, v64, table = kvc.cache(rng, int4, lens, hkv, hd, mb, B * mb)
+            z = np.zeros((B, hkv, mb * PAGE), np.float32)
+            cases.append((int4, B, hq, hkv, hd, mb, Held(
+                poor, q=rng.normal(0, 1, (B, hq, hd)).astype(np.float32), kp=kp, vp=vp, table=table, lens=np.array(lens, np.int32),
+                seen=np.array(lens, np.int32), out=np.zeros((B, hq, hd), np.float16), w=z, tags=z.astype(np.int32)), k64, v64, lens))
+    poor.limit(64)
+    for int4, B, hq, hkv, hd, mb, h, k64, v64, lens in cases:
+        f = poor.attn_decode_paged_int4 if int4 else poor.attn_decode_paged_f16_acc
+        f(h["q"], h["kp"], h["vp"], h["table"], h["lens"], h["out"], h["w"], B, hq, hkv, hd, mb, B * mb)
+        out = h.get("out").astype(np.float64)
+        for b, n in enumerate(lens):
+            want, _, A, e = attention(h.a["q"][b], in_order(k64, h.a["table"][b], n), in_order(v64, h.a["table"][b], n))
+            assert (np.abs(out[b] - want) <= 2.0**-11 * np.abs(want) + (e + 2.0**-18) * A + 2.0**-25).all()
+        keep = max(1, max(lens) // 2)
+        kvc.run_evict(poor, int4, h, B, hkv, hd, mb, B * mb, keep, 0, True)
+        assert h.get("lens").tolist() == [min(n, keep) for n in lens]
+    poor.limit(0)
+    for c in cases:
+        c[6].free()
