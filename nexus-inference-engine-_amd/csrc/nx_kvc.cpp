@@ -45,27 +45,36 @@ size_t pool_bytes(bool int4, int hkv, int hd, int num_blocks) {
     return (size_t)num_blocks * hkv * (int4 ? nx::kvc::page_bytes(hd) : 2 * nx::kPage * hd);
 }
 
-// The workspace of attention and eviction, grown when a call needs more.  In
-// a token batch the old one is kept until the batch has run, and the
+// The workspace of attention and eviction, grown when a call needs more: the
+// old one goes first, behind a wait for its last call.  In a token batch,
+// whose launches name the old one, it is kept until the batch has run, and the
 // allocation is declared as no part of the capture.
 nx_status kvc_ws(nx_ctx* ctx, size_t bytes, const char* name) {
     if (bytes <= ctx->kvc_ws_bytes) return NX_OK;
-    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-    if (ctx->capturing) NX_HIP(ctx, hipThreadExchangeStreamCaptureMode(&mode));
     void* ws = nullptr;
-    const hipError_t e = nx::dev_malloc(ctx, &ws, bytes);
-    if (ctx->capturing) (void)hipThreadExchangeStreamCaptureMode(&mode);
-    if (e != hipSuccess) return nx::hip_fail(ctx, e, name);
-    if (ctx->kvc_ws && ctx->capturing) {
-        try {
-            ctx->outgrown.push_back(ctx->kvc_ws);
-        } catch (...) {
-            (void)hipFree(ws);
-            return fail(ctx, NX_ERR_OOM, "%s: no memory for the list of old workspaces", name);
+    if (!ctx->capturing) {
+        if (ctx->kvc_ws) {
+            NX_HIP(ctx, hipStreamSynchronize(ctx->stream));
+            (void)hipFree(ctx->kvc_ws);
+            ctx->kvc_ws = nullptr;
+            ctx->kvc_ws_bytes = 0;
         }
-    } else if (ctx->kvc_ws) {
-        (void)hipStreamSynchronize(ctx->stream);
-        (void)hipFree(ctx->kvc_ws);
+        const hipError_t e = nx::dev_malloc(ctx, &ws, bytes);
+        if (e != hipSuccess) return nx::hip_fail(ctx, e, name);
+    } else {
+        if (ctx->kvc_ws) {
+            try {
+                ctx->outgrown.reserve(ctx->outgrown.size() + 1);
+            } catch (...) {
+                return fail(ctx, NX_ERR_OOM, "%s: no memory for the list of old workspaces", name);
+            }
+        }
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        NX_HIP(ctx, hipThreadExchangeStreamCaptureMode(&mode));
+        const hipError_t e = nx::dev_malloc(ctx, &ws, bytes);
+        (void)hipThreadExchangeStreamCaptureMode(&mode);
+        if (e != hipSuccess) return nx::hip_fail(ctx, e, name);
+        if (ctx->kvc_ws) ctx->outgrown.push_back(ctx->kvc_ws);
     }
     ctx->kvc_ws = ws;
     ctx->kvc_ws_bytes = bytes;

@@ -253,3 +253,41 @@ def test_reserved_calls_allocate_nothing(poor):
     poor.limit(0)
     for c in cases:
         c[6].free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capture", [False, True], ids=["eager", "captured"])
+def test_a_workspace_that_cannot_grow(poor, capture):
+    """A call without memory fails with NX_ERR_OOM; smaller ones run on, before
+    and after it, in the same token batch too."""
+    rng = np.random.default_rng(9)
+    small, big = [], []
+    for n, to in ((100, small), (30000, big)):
+        mb = -(-n // PAGE)
+        kp, vp, k64, v64, table = kvc.cache(rng, True, [n], 1, 64, mb, mb)
+        to += [n, mb, k64, v64, table, Held(poor, q=rng.normal(0, 1, (1, 8, 64)).astype(np.float32), kp=kp, vp=vp, table=table,
+                                            lens=np.array([n], np.int32), out=np.zeros((1, 8, 64), np.float16),
+                                            w=np.zeros((1, 1, mb * PAGE), np.float32))]
+
+    def attend_to(n, mb, k64, v64, table, h):
+        poor.attn_decode_paged_int4(h["q"], h["kp"], h["vp"], h["table"], h["lens"], h["out"], h["w"], 1, 8, 1, 64, mb, mb)
+
+    attend_to(*small)
+    poor.limit(1 << 16)
+    if capture:
+        poor.check(poor.L.nx_token_begin(poor.h), "begin")
+    with pytest.raises(kvc.nexus_amd.NxError) as e:
+        attend_to(*big)
+    assert e.value.code == 3
+    attend_to(*small)
+    if capture:
+        poor.check(poor.L.nx_token_end(poor.h), "end")
+    n, mb, k64, v64, table, h = small
+    want, W, A, e = attention(h.a["q"][0], in_order(k64, table[0], n), in_order(v64, table[0], n))
+    assert (np.abs(h.get("out")[0] - want) <= 2.0**-11 * np.abs(want) + (e + 2.0**-18) * A + 2.0**-25).all()
+    assert (np.abs(h.get("w")[0][:, :n] - 2 * W) <= 2 * (e + 2.0**-22) * W).all()
+    poor.limit(0)
+    attend_to(*big)
+    assert abs(big[5].get("w").sum() - 8) < 1e-3
+    for x in (small, big):
+        x[5].free()
