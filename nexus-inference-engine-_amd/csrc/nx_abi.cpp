@@ -151,6 +151,7 @@ void tq_codebook(int d, int bits, float* c, float* bnd) {
 namespace nx {
 hipError_t dev_malloc(nx_ctx* ctx, void** p, size_t bytes) {
     *p = nullptr;
+    if (ctx->device < 0) return hipErrorNoDevice;
     // (more than any device has, so that the failure is the runtime's own)
     const size_t ask = ctx->alloc_limit && bytes > ctx->alloc_limit ? (size_t)1 << 60 : bytes;
     hipError_t e = hipMalloc(p, ask);
@@ -169,13 +170,18 @@ extern "C" {
 void nx_limit_allocations(nx_ctx* ctx, size_t bytes) { ctx->alloc_limit = bytes; }
 
 // Not part of the interface: a context without a device, whose buffers (ids
-// 1 .. n of the given sizes) are numbers alone, to test what calls refuse
-// before they reach a device.
+// 1 .. n of the given sizes) are numbers alone, to test what the compact
+// cache's calls refuse before they reach a device.  Other calls do not know them.
 nx_ctx* nx_deviceless(const size_t* bytes, int n) {
     nx_ctx* ctx = new (std::nothrow) nx_ctx();
     if (!ctx) return nullptr;
     ctx->device = -1;
-    for (int i = 0; i < n; ++i) ctx->bufs[(uint64_t)i + 1] = bytes[i];
+    try {
+        for (int i = 0; i < n; ++i) ctx->numbers[(uint64_t)i + 1] = bytes[i];
+    } catch (...) {
+        delete ctx;
+        return nullptr;
+    }
     return ctx;
 }
 
@@ -279,6 +285,7 @@ nx_status nx_alloc(nx_ctx* ctx, size_t bytes, nx_buf* out) {
     if (!ctx || !out) return NX_ERR_INVALID;
     if (bytes == 0) return fail(ctx, NX_ERR_INVALID, "nx_alloc: zero bytes");
     if (ctx->capturing) return fail(ctx, NX_ERR_STATE, "nx_alloc inside a token batch");
+    if (ctx->device < 0) return fail(ctx, NX_ERR_NO_DEVICE, "nx_alloc: no device");
     void* p = nullptr;
     hipError_t e = nx::dev_malloc(ctx, &p, bytes);
     if (e != hipSuccess) return nx::hip_fail(ctx, e, "hipMalloc");
@@ -409,6 +416,7 @@ nx_status nx_clear_buffer_cache(nx_ctx* ctx) {
 
 nx_status nx_synchronize(nx_ctx* ctx) {
     if (!ctx) return NX_ERR_INVALID;
+    if (ctx->device < 0) return fail(ctx, NX_ERR_NO_DEVICE, "nx_synchronize: no device");
     NX_HIP(ctx, hipStreamSynchronize(ctx->stream));
     return NX_OK;
 }
@@ -416,6 +424,7 @@ nx_status nx_synchronize(nx_ctx* ctx) {
 // ----------------------------------------------------------------- batching --
 nx_status nx_token_begin(nx_ctx* ctx) {
     if (!ctx) return NX_ERR_INVALID;
+    if (ctx->device < 0) return fail(ctx, NX_ERR_NO_DEVICE, "nx_token_begin: no device");
     if (ctx->capturing || ctx->token_flushed) return fail(ctx, NX_ERR_STATE, "token batch already open");
     NX_HIP(ctx, hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeThreadLocal));
     ctx->capturing = true;

@@ -18,6 +18,7 @@ struct nx_ctx {
     hipStream_t stream = nullptr;
     std::map<uint64_t, size_t> bufs;                   // device address -> bytes
     std::set<uint64_t> wrapped;                        // those of bufs whose memory is the caller's
+    std::map<uint64_t, size_t> numbers;                // nx_deviceless: "buffers" without memory
     std::unordered_map<const void*, uint64_t> wcache;  // host key -> buffer
     std::string err;
     bool capturing = false;

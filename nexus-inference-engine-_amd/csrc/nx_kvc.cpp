@@ -16,6 +16,22 @@ T* dptr(nx_buf b) {
     return reinterpret_cast<T*>(static_cast<uintptr_t>(b));
 }
 
+// NX_NEED, which knows the numbers of a context without a device as well: these
+// calls end before they would be taken for addresses.
+nx_status need(nx_ctx* ctx, nx_buf b, size_t bytes, const char* name) {
+    if (ctx->device >= 0 || !ctx->numbers.count(b)) {
+        NX_NEED(ctx, b, bytes, name);
+        return NX_OK;
+    }
+    const size_t has = ctx->numbers[b];
+    return has < bytes ? fail(ctx, NX_ERR_INVALID, "%s: buffer has %zu bytes, needs %zu", name, has, bytes) : NX_OK;
+}
+#define NEED(ctx, b, bytes, name)                                  \
+    do {                                                           \
+        const nx_status nx_s_ = need((ctx), (b), (bytes), (name)); \
+        if (nx_s_ != NX_OK) return nx_s_;                          \
+    } while (0)
+
 // The context's device for the time of a call.
 struct OnDevice {
     int before = -1;
@@ -94,12 +110,12 @@ nx_status rows_int4(nx_ctx* ctx, const char* name, bool append, nx_buf k, nx_buf
     if (tokens > max_blocks * nx::kPage)
         return fail(ctx, NX_ERR_CAPACITY, "%s: %d tokens exceed %d blocks of %d", name, tokens, max_blocks, nx::kPage);
     const size_t rows = (size_t)batch * tokens * hkv * hd * 4, pool = pool_bytes(true, hkv, hd, num_blocks);
-    NX_NEED(ctx, k, rows, "k");
-    NX_NEED(ctx, v, rows, "v");
-    NX_NEED(ctx, kpool, pool, "kpool");
-    NX_NEED(ctx, vpool, pool, "vpool");
-    NX_NEED(ctx, bt, (size_t)batch * max_blocks * 4, "block_table");
-    NX_NEED(ctx, pos, (size_t)batch * 4, "positions");
+    NEED(ctx, k, rows, "k");
+    NEED(ctx, v, rows, "v");
+    NEED(ctx, kpool, pool, "kpool");
+    NEED(ctx, vpool, pool, "vpool");
+    NEED(ctx, bt, (size_t)batch * max_blocks * 4, "block_table");
+    NEED(ctx, pos, (size_t)batch * 4, "positions");
     const nx_buf all[] = {k, v, kpool, vpool, bt, pos}, outs[] = {append ? kpool : k, append ? vpool : v};
     for (nx_buf o : outs) {
         int n = 0;
@@ -133,13 +149,13 @@ nx_status attn_kvc(nx_ctx* ctx, const char* name, bool int4, nx_buf q, nx_buf kp
     if (hq < 1 || hq % hkv) return fail(ctx, NX_ERR_INVALID, "%s: hq %d is no multiple of hkv %d", name, hq, hkv);
     if (hq / hkv > kMaxGroup) return fail(ctx, NX_ERR_UNSUPPORTED, "%s: hq/hkv = %d above %d", name, hq / hkv, kMaxGroup);
     const size_t pool = pool_bytes(int4, hkv, hd, num_blocks);
-    NX_NEED(ctx, q, (size_t)batch * hq * hd * 4, "q");
-    NX_NEED(ctx, kpool, pool, "kpool");
-    NX_NEED(ctx, vpool, pool, "vpool");
-    NX_NEED(ctx, bt, (size_t)batch * max_blocks * 4, "block_table");
-    NX_NEED(ctx, lens, (size_t)batch * 4, "ctx_lens");
-    NX_NEED(ctx, out, (size_t)batch * hq * hd * 2, "out");
-    if (weights || !int4) NX_NEED(ctx, weights, (size_t)batch * hkv * max_blocks * nx::kPage * 4, "weights");
+    NEED(ctx, q, (size_t)batch * hq * hd * 4, "q");
+    NEED(ctx, kpool, pool, "kpool");
+    NEED(ctx, vpool, pool, "vpool");
+    NEED(ctx, bt, (size_t)batch * max_blocks * 4, "block_table");
+    NEED(ctx, lens, (size_t)batch * 4, "ctx_lens");
+    NEED(ctx, out, (size_t)batch * hq * hd * 2, "out");
+    if (weights || !int4) NEED(ctx, weights, (size_t)batch * hkv * max_blocks * nx::kPage * 4, "weights");
     const nx_buf in[] = {q, kpool, vpool, bt, lens};
     bool clash = out == weights;
     for (nx_buf b : in) clash = clash || b == out || (weights && b == weights);
@@ -177,16 +193,16 @@ nx_status evict(nx_ctx* ctx, const char* name, bool int4, nx_buf kpool, nx_buf v
     if (keep < 1 || recent < 0 || recent > keep)
         return fail(ctx, NX_ERR_INVALID, "%s: keep %d must be positive and recent %d within it", name, keep, recent);
     const size_t pool = pool_bytes(int4, hkv, hd, num_blocks), slots = (size_t)batch * hkv * max_blocks * nx::kPage * 4;
-    NX_NEED(ctx, kpool, pool, "kpool");
-    NX_NEED(ctx, vpool, pool, "vpool");
-    NX_NEED(ctx, bt, (size_t)batch * max_blocks * 4, "block_table");
-    NX_NEED(ctx, lens_in, (size_t)batch * 4, "ctx_lens");
-    NX_NEED(ctx, seen, (size_t)batch * 4, "seen");
-    NX_NEED(ctx, w_in, slots, "weights");
-    NX_NEED(ctx, t_in, slots, "tags");
-    NX_NEED(ctx, lens_out, (size_t)batch * 4, "lens_out");
-    NX_NEED(ctx, w_out, slots, "weights_out");
-    NX_NEED(ctx, t_out, slots, "tags_out");
+    NEED(ctx, kpool, pool, "kpool");
+    NEED(ctx, vpool, pool, "vpool");
+    NEED(ctx, bt, (size_t)batch * max_blocks * 4, "block_table");
+    NEED(ctx, lens_in, (size_t)batch * 4, "ctx_lens");
+    NEED(ctx, seen, (size_t)batch * 4, "seen");
+    NEED(ctx, w_in, slots, "weights");
+    NEED(ctx, t_in, slots, "tags");
+    NEED(ctx, lens_out, (size_t)batch * 4, "lens_out");
+    NEED(ctx, w_out, slots, "weights_out");
+    NEED(ctx, t_out, slots, "tags_out");
     // What is written is no other buffer of the call, but that each of the last
     // three may be the input of its kind.  (The places count: an input that is
     // given twice may not be one output's own and stand for another input.)

@@ -291,3 +291,21 @@ def test_a_workspace_that_cannot_grow(poor, capture):
     assert abs(big[5].get("w").sum() - 8) < 1e-3
     for x in (small, big):
         x[5].free()
+
+
+# ------------------------------------------------- a context without a device --
+def test_only_the_calls_it_is_for_know_its_buffers():
+    """The buffers of a context without a device are numbers, not addresses: every
+    call but the compact cache's refuses them, and nothing is allocated for it."""
+    L = kvc.nexus_amd.lib()
+    L.nx_deviceless.restype = kvc.C.c_void_p
+    ctx = kvc.C.c_void_p(L.nx_deviceless((kvc.C.c_size_t * 3)(1 << 20, 1 << 20, 1 << 20), 3))
+    host = np.zeros(64, np.float32)
+    size, buf = kvc.C.c_size_t(), kvc.C.c_uint64()
+    for status in (L.nx_residual_add(ctx, 1, 2, 3, 16), L.nx_download(ctx, host.ctypes.data, 1, 0, 64), L.nx_upload(ctx, 1, 0, host.ctypes.data, 64),
+                   L.nx_argmax(ctx, 1, 2, 16, 1), L.nx_free(ctx, 1), L.nx_buffer_size(ctx, 1, kvc.C.byref(size))):
+        assert status == 1 and b"unknown buffer" in L.nx_last_error(ctx)
+    assert L.nx_alloc(ctx, 64, kvc.C.byref(buf)) == 6 and buf.value == 0
+    assert L.nx_token_begin(ctx) == 6 and L.nx_synchronize(ctx) == 6
+    assert call("nx_kv_append_int4", [1, 2, 3, 4, 5, 6], kvc.SHAPE)[0] == 6
+    L.nx_destroy(ctx)
