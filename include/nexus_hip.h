@@ -254,7 +254,8 @@ nx_status nx_attn_decode_paged_tq(nx_ctx* ctx, nx_buf q_f32, nx_buf kc4, nx_buf 
  * reads back as NaN.  Rows of a sequence that would begin below 0 or end
  * beyond max_blocks * 16 are not written, nor are rows whose table entry lies
  * outside [0, num_blocks).  tokens beyond max_blocks * 16: NX_ERR_CAPACITY.
- * Two sequences must not write to one page.  hkv up to 4096, batch up to
+ * No two rows may go to one place, so no page may belong to two sequences, or
+ * twice to one.  hkv up to 4096, batch up to
  * 65535, max_blocks up to 2^22, as for the calls below. */
 nx_status nx_kv_append_int4(nx_ctx* ctx, nx_buf k_f32, nx_buf v_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
                             nx_buf positions_i32, int batch, int tokens, int hkv, int head_dim, int max_blocks,

@@ -10,9 +10,10 @@
 // k_pick, one block per (sequence, kv head): a radix selection over 32-bit
 // keys (11, 11 and 10 bits), which stay in LDS, finds the keep-th largest;
 // ballots number the equal ones, the free slots and the tokens that move in
-// slot order.  k_move, one wavefront per destination page:
-// weights and tags; K vectors as they are; V, whose pages are dimension-major,
-// by rewriting the page's words, each of which one lane owns.
+// slot order.  k_move, a wavefront per destination page of int4 pages and 1 + hd /
+// 64 of fp16 ones (K, and 64 dimensions of V each): weights and tags; K vectors
+// as they are; V, whose pages are dimension-major, by rewriting the page's words
+// (fp16: half rows of eight tokens), each of which one lane owns.
 #include <algorithm>
 
 #include "nx_kvc.h"

@@ -84,7 +84,7 @@ struct Eight {
 
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void k_append_int4(RowArgs a) {
-    constexpr int S = HD / 32, C = HD / 8;
+    constexpr int C = HD / 8;
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const RowPage pr = row_page(a.start[b], a.tokens, a.max_blocks, blockIdx.x);
     if (pr.none || pr.refused) return;
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(2 * HD) void k_append_int4(RowArgs a) {
     *reinterpret_cast<uint2*>(codes + t * HD + 8 * c) = make_uint2(w2[0], w2[1]);
     __syncthreads();
     // thread tid owns dword tid of V: tokens 4 g + j of dimensions d and d + 16
-    const int i = tid % S, n = (tid / S) % 16, g = tid / S / 16, d = 32 * i + n;
+    const int g = v_word(HD, tid).g, d = v_word(HD, tid).d;
     uint32_t out = 0u, mask = 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(2 * HD) void k_append_int4(RowArgs a) {
 // whole lines (with eight of one token 4096 tokens took 14.0 us in place of 12.3).
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void k_read_int4(RowArgs a) {
-    constexpr int S = HD / 32, C = HD / 4;
+    constexpr int C = HD / 4;
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const RowPage pr = row_page(a.start[b], a.tokens, a.max_blocks, blockIdx.x);
     if (pr.none) return;
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(2 * HD) void k_read_int4(RowArgs a) {
         wk[u] = reinterpret_cast<const uint32_t*>(a.kpool + rec)[k_word(HD, t, 4 * c)] >> (c % 2 * 8);
     }
     __shared__ uint8_t codes[kPage * HD];
-    const int i = tid % S, n = (tid / S) % 16, g = tid / S / 16, d = 32 * i + n;
+    const int g = v_word(HD, tid).g, d = v_word(HD, tid).d;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll

@@ -1,7 +1,8 @@
 // Entry points of the compact KV cache (nx_kvc.h): checks of shapes and
 // buffers on the host, the workspace, the launches.  Lengths, positions and
 // block tables are checked by the kernels, so no call waits for the device
-// and every call may be captured into a token batch.
+// (but where its workspace grows outside a token batch) and every call may be
+// captured into a token batch.
 #include <algorithm>
 
 #include "nx_internal.h"

@@ -26,7 +26,11 @@ namespace kvc {
 __host__ __device__ constexpr int page_bytes(int hd) { return 9 * hd; }
 __host__ __device__ constexpr int k_word(int hd, int t, int d) { return t * (hd / 8) + ((d >> 3) & 3) * (hd / 32) + (d >> 5); }
 __host__ __device__ constexpr int k_nib(int d) { return ((d & 7) >> 1) + 4 * (d & 1); }
-__host__ __device__ constexpr int v_word(int hd, int t, int d) { return (16 * (t >> 2) + (d & 15)) * (hd / 32) + (d >> 5); }
+// what V's dword w holds: tokens 4 g .. + 3 of dimensions d and d + 16
+struct VWord {
+    int g, d;
+};
+__host__ __device__ constexpr VWord v_word(int hd, int w) { return {w / (hd / 32) / 16, 32 * (w % (hd / 32)) + w / (hd / 32) % 16}; }
 __host__ __device__ constexpr int v_nib(int t, int d) { return ((t & 3) >> 1) + 2 * ((d >> 4) & 1) + 4 * (t & 1); }
 // index of a scale among the page's halves: the four tokens of a lane together
 __host__ __device__ constexpr int scale_at(int hd, int t, int grp) { return ((t >> 2) * (hd / 32) + grp) * 4 + (t & 3); }
