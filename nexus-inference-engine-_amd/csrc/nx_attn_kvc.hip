@@ -24,10 +24,11 @@
 //
 // int4-g32: a step of 32 dimensions is one scale group, so codes enter the
 // products as exact fp16 integers and the scales stay outside: fp32 behind K's
-// product, in front of V's with the probability.  Bound by the vector
-// instructions beside the products (about 300 a pair of pages of 128 dimensions)
-// and, one pair to a wavefront, by latency: 32768 tokens of 8 kv heads (38 MB)
-// 11.4 us and a join of 3.9.
+// product, in front of V's with the probability.  Between two bounds: vector
+// instructions beside the products (356 a pair of pages of 128 dimensions, 275
+// more a wavefront) take 57 % of the SIMDs' time, and a wavefront, which has half
+// a pair in flight, waits for memory in 48 % of its own: 32768 tokens of 8 kv heads
+// (38 MB) 12.6 us and a join of 3.9.
 #include <algorithm>
 #include <type_traits>
 
@@ -756,10 +757,10 @@ AttnPlan attn_plan(int batch, int hq, int hkv, int hd, int max_blocks, bool int4
     // 1.4 us (fp16) per 64 dimensions, 15 % less where it holds two blocks at
     // once, 0.4 of that and up for fewer than eight pairs; 3 us and a little per
     // split for records and join, or without a join half a microsecond for eight
-    // pairs' weights.  (8 kv heads of 128, int4: 512 tokens 6.6 us in one block
-    // each and 7.7 in eight with a join, 1024 tokens 9.7 and 7.9; 8 sequences of
-    // 8192 21.2 us in four, 18.9 in eight; 6 of 2500, 8 heads of 64, fp16: 11.0 us
-    // in four, 11.9 in ten.)
+    // pairs' weights.  (8 kv heads of 128, int4: 512 tokens 6.9 us in one block
+    // each and 8.5 in eight with a join, 1024 tokens 10.1 and 8.5; 8 sequences of
+    // 8192 21.2 us in four, 19.5 in eight; 6 of 2500, 8 heads of 64, fp16: 11.5 us
+    // in five, 12.8 in twelve.)
     const int64_t rows = (int64_t)batch * hkv * p.groups, cus = device_cus(), pair = (int4 ? 80 : 140) * (hd / 64);
     const bool joined = weights && p.groups > 1, two = hd * (int4 ? 1 : 2) <= 128;
     int64_t least = INT64_MAX;

@@ -110,7 +110,7 @@ __device__ inline int2 block_scan(int2 v, int2* lds, int2& total) {
 // others by its instructions.  A row's slots are passed three times: keys and
 // their top bits are counted, the keys of the bin that holds the keep-th are
 // listed, and the keys are compared with the keep-th (twice more where some of
-// its equals stay and some go).  8 kv heads of 32768 slots: 17.5 us, of 4352: 8.3 us.
+// its equals stay and some go).  8 kv heads of 32768 slots: 18.0 us, of 4352: 8.2 us.
 template <int SLOTS>
 __global__ __launch_bounds__(kPickThreads) void k_pick(EvictArgs a) {
     // two counters per bin, by lane: weights crowd into few bins
@@ -517,7 +517,7 @@ __device__ inline void move_int4(const EvictArgs& a, size_t dst, size_t src, int
 // token leaves is cleared by the lane that has read it, every other by its own.
 // fp16: bound by memory, since V's pages are dimension-major, so that a token
 // moves with whole pages: 8 sequences of 8192 tokens of 8 kv heads of 128 cut to
-// 2048 read 173 MB and write 65, 51.5 us; int4, one of 32768 cut to 4096: 7.7 us.
+// 2048 read 173 MB and write 65, 51 us; int4, one of 32768 cut to 4096: 8.0 us.
 template <int HD, bool INT4>
 constexpr int kParts = INT4 ? 1 : 1 + HD / kWave;  // wavefronts of a page
 

@@ -343,7 +343,9 @@ class Context:
         self.check(self.L.nx_gemv_int4_g32_f32(self.h, x, wq, sc, y, N, K, batch, int(accumulate)),
                    "nx_gemv_int4_g32_f32")
 
-    # the compact KV cache (include/nexus_hip.h); buffers are handles
+    # the compact KV cache (include/nexus_hip.h); buffers are handles.  Calls are
+    # queued on the context's stream, which other libraries' streams know nothing
+    # of: sync() (or download(), which waits) before what they write is read there.
     def reserve_kv_compact(self, batch, hq, hkv, head_dim, max_ctx):
         self.check(self.L.nx_reserve_kv_compact(self.h, batch, hq, hkv, head_dim, max_ctx), "nx_reserve_kv_compact")
 
