@@ -255,8 +255,8 @@ nx_status nx_attn_decode_paged_tq(nx_ctx* ctx, nx_buf q_f32, nx_buf kc4, nx_buf 
  * beyond max_blocks * 16 are not written, nor are rows whose table entry lies
  * outside [0, num_blocks).  tokens beyond max_blocks * 16: NX_ERR_CAPACITY.
  * No two rows may go to one place, so no page may belong to two sequences, or
- * twice to one.  hkv up to 4096, batch up to
- * 65535, max_blocks up to 2^22, as for the calls below. */
+ * twice to one.  hkv up to 4096, batch up to 65535, max_blocks up to 2^22, as
+ * for the calls below. */
 nx_status nx_kv_append_int4(nx_ctx* ctx, nx_buf k_f32, nx_buf v_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
                             nx_buf positions_i32, int batch, int tokens, int hkv, int head_dim, int max_blocks,
                             int num_blocks);
@@ -277,7 +277,8 @@ nx_status nx_kv_read_int4(nx_ctx* ctx, nx_buf kpool, nx_buf vpool, nx_buf block_
  * weights stay as they are.  A cached value of its positions that is not
  * finite shows: K's makes its kv head's rows and weights NaN, V's makes its
  * dimension (of int4 pages its group) NaN or infinite; one of q makes its head's
- * row and the kv head's weights NaN.  Slots past the length may hold anything.  No output or weights buffer may be another buffer of the call. */
+ * row and the kv head's weights NaN.  Slots past the length may hold anything.
+ * No output or weights buffer may be another buffer of the call. */
 nx_status nx_attn_decode_paged_int4(nx_ctx* ctx, nx_buf q_f32, nx_buf kpool, nx_buf vpool, nx_buf block_table,
                                     nx_buf ctx_lens_i32, nx_buf out_f16, nx_buf weights_f32, int batch, int hq, int hkv,
                                     int head_dim, int max_blocks, int num_blocks);

@@ -274,20 +274,26 @@ template <int HD>
 __device__ inline float most_up(const PairI4<HD>& r, float up) {
     typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
     typedef uint16_t us4_t __attribute__((ext_vector_type(4)));
-    auto most = [&](uint16_t bits) {  // of the scales, each masked
+    auto most = [&](auto&& of) {  // of the scales' bits
         us2_t m = {0, 0};
 #pragma unroll
         for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
-                const us4_t w = __builtin_bit_cast(us4_t, r.vs[pg][i]) & bits;
+                const us4_t w = of(__builtin_bit_cast(us4_t, r.vs[pg][i]));
                 m = __builtin_elementwise_max(m, __builtin_elementwise_max(__builtin_shufflevector(w, w, 0, 1), __builtin_shufflevector(w, w, 2, 3)));
             }
-        return max((int)m.x, (int)m.y) >> 10;  // biased exponent: 15 is 2^0 (and 32 and up: a negative one)
+        return max((int)m.x, (int)m.y) >> 10;  // biased exponent: 15 is 2^0
     };
     constexpr int kTop = 14 + (int)kUp;
-    if (!__any(most(0xFFFFu) > kTop - (int)up)) return up;
-    return fminf(up, (float)kTop - wave_max((float)most(0x7FFFu)));
+    // (a negative scale's is 32 and up, one's that is not finite 31: these are
+    // looked at again, the sign off, and no factor makes the latter's products finite)
+    if (!__any(most([](us4_t w) { return w; }) > kTop - (int)up)) return up;
+    const int e = most([](us4_t w) {
+        const us4_t size = w & (uint16_t)0x7FFFu;
+        return size & __builtin_bit_cast(us4_t, size < (uint16_t)0x7C00u);
+    });
+    return fminf(up, (float)kTop - wave_max((float)e));
 }
 template <int HD>
 __device__ inline float most_up(const PairF16<HD>&, float up) {

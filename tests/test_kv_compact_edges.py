@@ -177,6 +177,30 @@ def test_an_infinite_scale_of_int4_pages(ctx, hd, value):
     assert np.isfinite(out[8:]).all() and abs(w[1].sum() - 8) < 1e-4
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_a_value_that_is_not_finite_costs_the_other_groups_nothing(ctx, hd, value):
+    """The heaviest token of every pair of pages holds a NaN or an infinity in its
+    first group and zeros elsewhere, the others, of 2^-17 of its weight, ones: they
+    are what the other groups' outputs consist of, as exact as without the first
+    group (test_probabilities_keep_more_than_fp16; 31 2^-17 is 2^-12)."""
+    n = 512
+    k, v = np.zeros((n, 1, hd), np.float32), np.ones((n, 1, hd), np.float32)
+    k[::2 * PAGE, 0, 0] = 17 * np.log(2) * np.sqrt(hd)
+    v[::2 * PAGE, 0] = 0
+    v[::2 * PAGE, 0, 3] = value
+    kp, vp, k64, v64, table = one_sequence(np.random.default_rng(hd), k, v, n // PAGE)
+    q = np.zeros((1, hd))
+    q[0, 0] = 1
+    out, _ = attend(ctx, q, kp, vp, table, n)
+    assert np.isnan(out[:, :32]).all()
+    want, W, A, _ = attention(q, k64, v64)
+    assert (np.abs(want[:, 32:] * 2**12 - 1) < 0.05).all()
+    e = 6 * 2.0**-24 * 17 + 2.0**-19
+    assert (np.abs(out - want) <= 2.0**-11 * np.abs(want) + (e + 2.0**-19) * A + n * 2.0**-33 + 2.0**-25)[:, 32:].all()
+
+
 # ------------------------------------------------------------ shared buffers --
 @pytest.mark.parametrize("op", ["nx_kv_evict_f16", "nx_kv_evict_int4"])
 def test_eviction_refuses_pools_that_are_another_buffer(op):
