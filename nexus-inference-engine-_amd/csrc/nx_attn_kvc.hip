@@ -113,6 +113,13 @@ __device__ inline void load_scales(h4_t (&r)[N], const uint8_t* p) {
     }
 }
 
+// (Kept apart from the page's address, which is the same in all lanes: as sums
+// of 64 bits the four addresses would take eight registers over the loop.)
+__device__ inline uint32_t lane_offset(uint32_t v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 template <int HD>
 __device__ inline void load_k(PairI4<HD>& r, const AttnArgs& a, const int (&blk)[2], int kvh, int lane) {
     constexpr int S = HD / 32;
@@ -120,8 +127,8 @@ __device__ inline void load_k(PairI4<HD>& r, const AttnArgs& a, const int (&blk)
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
         const uint8_t* p = a.kpool + ((size_t)(uint32_t)blk[pg] * (uint32_t)a.hkv + (uint32_t)kvh) * page_bytes(HD);
-        load_words<S>(r.k[pg], p + (t * 4 + g) * (4 * S));
-        load_scales<S>(r.ks[pg], p + 8 * HD + g * (8 * S));
+        load_words<S>(r.k[pg], p + lane_offset((t * 4 + g) * (4 * S)));
+        load_scales<S>(r.ks[pg], p + 8 * HD + lane_offset(g * (8 * S)));
     }
 }
 template <int HD>
@@ -130,8 +137,8 @@ __device__ inline void load_v(PairI4<HD>& r, const AttnArgs& a, const int (&blk)
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
         const uint8_t* p = a.vpool + ((size_t)(uint32_t)blk[pg] * (uint32_t)a.hkv + (uint32_t)kvh) * page_bytes(HD);
-        load_words<S>(r.v[pg], p + (uint32_t)lane * (4 * S));
-        load_scales<S>(r.vs[pg], p + 8 * HD + ((uint32_t)lane >> 4) * (8 * S));
+        load_words<S>(r.v[pg], p + lane_offset((uint32_t)lane * (4 * S)));
+        load_scales<S>(r.vs[pg], p + 8 * HD + lane_offset(((uint32_t)lane >> 4) * (8 * S)));
     }
 }
 
@@ -254,51 +261,71 @@ __device__ inline void clear_past(PairF16<HD>& r, int na, int nb, int lane) {
 // fp16 numbers (below 2^-14 fp16 loses bits); L and O have the same factor.
 // The reference is the first pair's maximum and follows a larger one only when
 // that is more than 2^kLead ahead (kUp + kLead is 15): O is hardly ever
-// multiplied through.
+// multiplied through.  int4 pages: `up` is kUp less what large scales ask for, and
+// O of a group of 32 dimensions has 2^(kUp - down) in place of 2^up (make_room; the
+// same in all lanes).
 template <int HD>
 struct Fold {
     float m = -__builtin_inff(), l = 0.0f, up = kUp;
+    int down[HD / 32] = {};
     f4_t o[HD / 16];
 };
 
 // ------------------------------------------------------------ values of a pair --
-// The powers of two that a pair's probabilities may have.  P V takes p
-// times the token's scale as fp16 numbers (below).  p is 2^15 at most, and as
-// much more as the roundings of scores below kFar give (2^-4 in the exponent
-// at 2^20), so with a scale of 1 or more (a value of 8 and up among a group) the
-// product could pass the largest fp16 number: from such a pair on the
-// wavefront's factor is as many powers of two smaller, down to 2^-5.  (What fp16's
-// smallest number, 2^-24, then leaves out of a token's term is 2^-34 of the largest
-// |V| among the wavefront's tokens.)
+// P V takes p times the token's scale as fp16 numbers (below).  p is 2^15 at
+// most, and as much more as the roundings of scores below kFar give (a tenth in
+// the exponent), so with a scale of 1 or more (a value of 8 and up among a
+// group) the product could pass the largest fp16 number: from such a pair on
+// the wavefront's products for that group go without as many powers of two,
+// `down`.  Half of the most that a group asks for is taken from p, for all, and the
+// rest from (or back to) the scales, so that neither loses bits to fp16's smallest
+// number.  What that leaves out of a token's term is 2^-34 of the group's largest |V|
+// among the wavefront's tokens and 2^-28 of its own.
 template <int HD>
-__device__ inline float most_up(const PairI4<HD>& r, float up) {
+__device__ inline void make_room(Fold<HD>& f, PairI4<HD>& r) {
     typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
     typedef uint16_t us4_t __attribute__((ext_vector_type(4)));
-    auto most = [&](auto&& of) {  // of the scales' bits
-        us2_t m = {0, 0};
+    us2_t any = {0, 0};
 #pragma unroll
-        for (int pg = 0; pg < 2; ++pg)
+    for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
-                const us4_t w = of(__builtin_bit_cast(us4_t, r.vs[pg][i]));
-                m = __builtin_elementwise_max(m, __builtin_elementwise_max(__builtin_shufflevector(w, w, 0, 1), __builtin_shufflevector(w, w, 2, 3)));
-            }
-        return max((int)m.x, (int)m.y) >> 10;  // biased exponent: 15 is 2^0
-    };
-    constexpr int kTop = 14 + (int)kUp;
-    // (a negative scale's is 32 and up, one's that is not finite 31: these are
-    // looked at again, the sign off, and no factor makes the latter's products finite)
-    if (!__any(most([](us4_t w) { return w; }) > kTop - (int)up)) return up;
-    const int e = most([](us4_t w) {
-        const us4_t size = w & (uint16_t)0x7FFFu;
-        return size & __builtin_bit_cast(us4_t, size < (uint16_t)0x7C00u);
-    });
-    return fminf(up, (float)kTop - wave_max((float)e));
+        for (int i = 0; i < HD / 32; ++i) {
+            const us4_t w = __builtin_bit_cast(us4_t, r.vs[pg][i]);
+            any = __builtin_elementwise_max(any, __builtin_elementwise_max(__builtin_shufflevector(w, w, 0, 1), __builtin_shufflevector(w, w, 2, 3)));
+        }
+    // biased exponents: 15 is 2^0 (31 no number, 32 and up a negative one's)
+    if (!__any(max((int)any.x, (int)any.y) >= 15 << 10) && f.up == kUp) return;
+    int top = 0;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+        us4_t most = {0, 0, 0, 0};
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
+            const us4_t size = __builtin_bit_cast(us4_t, r.vs[pg][i]) & (uint16_t)0x7FFFu;
+            most = __builtin_elementwise_max(most, size & __builtin_bit_cast(us4_t, size < (uint16_t)0x7C00u));  // (no factor makes the others' products finite)
+        }
+        const int e = max(max((int)most[0], (int)most[1]), max((int)most[2], (int)most[3])) >> 10;
+        const int d = max(f.down[i], __builtin_amdgcn_readfirstlane((int)wave_max((float)e)) - 14);
+        const float by = ldexpf(1.0f, f.down[i] - d);
+        f.o[2 * i] *= by;
+        f.o[2 * i + 1] *= by;
+        f.down[i] = d;
+        top = max(top, d);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    const int half = (top + 1) / 2;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+        const _Float16 by = (_Float16)ldexpf(1.0f, half - f.down[i]);  // 2^-8 to 2^8
+        r.vs[0][i] *= h4_t{by, by, by, by};
+        r.vs[1][i] *= h4_t{by, by, by, by};
+    }
+    const float up = kUp - (float)half;
+    f.l *= __builtin_amdgcn_exp2f(up - f.up);
+    f.up = up;
 }
 template <int HD>
-__device__ inline float most_up(const PairF16<HD>&, float up) {
-    return up;
-}
+__device__ inline void make_room(Fold<HD>&, const PairF16<HD>&) {}
 
 // The lanes of columns 8-15 (those with bit 3), which hold the same
 // probabilities as columns 0-7: rows 0-7 of a product take the fp16 high parts
@@ -442,8 +469,9 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, const f4_t* off
     const bool far = fabsf(top) > kFar && top != -__builtin_inff();  // (of a column: heads go by their own scores)
     const float mn = top > (far ? f.m : f.m + kLead) ? top : f.m;
     const bool none = mn == -__builtin_inff();  // no token, or NaN scores alone
-    const float up = most_up<HD>(r, f.up);
-    const float corr = none ? 1.0f : __builtin_amdgcn_exp2f(f.m - mn + (up - f.up));
+    make_room<HD>(f, r);
+    const float up = f.up;
+    const float corr = none ? 1.0f : __builtin_amdgcn_exp2f(f.m - mn);
     float by = scale, from = none ? 0.0f : mn - up, sum = 0.0f;
     if (__any(far)) {
 #pragma unroll
@@ -469,7 +497,6 @@ __device__ inline void fold(Fold<HD>& f, Pair& r, const h8_t* q, const f4_t* off
             for (int j = 0; j < 4; ++j) f.o[nt][j] *= c[j];
     }
     f.m = mn;
-    f.up = up;
     values<HD>(r, p, f.o, lane);
 }
 
@@ -565,8 +592,7 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
         fold_all();
         if (mine > 0) use(mine - 1, [] {});
     }
-    const float factor = __builtin_amdgcn_exp2f(kUp - f.up);  // records have 2^kUp
-    const float l = sum_x32(sum_x16(f.l)) * factor;
+    const float l = ldexpf(sum_x32(sum_x16(f.l)), (int)(kUp - f.up));  // records have 2^kUp
     // rows 8-15 onto rows 0-7: tile 2 k's sums in the lower half of the lanes, tile
     // 2 k + 1's in the upper
 #pragma unroll
@@ -579,7 +605,7 @@ __global__ __launch_bounds__(kThreads, HD * (INT4 ? 1 : 2) <= 128 ? 4 : 2) void 
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) my[(4 * (g & 1) + j) * HD + 32 * i + 16 * (g >> 1) + t] = f.o[i][j] * factor;
+        for (int j = 0; j < 4; ++j) my[(4 * (g & 1) + j) * HD + 32 * i + 16 * (g >> 1) + t] = ldexpf(f.o[i][j], f.down[i]);
     if (lane < kHeadsPerBlock) {
         // M is NaN where the length or the table is out of range
         my[MO + lane] = bad ? __builtin_nanf("") : f.m;

@@ -201,6 +201,65 @@ def test_a_value_that_is_not_finite_costs_the_other_groups_nothing(ctx, hd, valu
     assert (np.abs(out - want) <= 2.0**-11 * np.abs(want) + (e + 2.0**-19) * A + n * 2.0**-33 + 2.0**-25)[:, 32:].all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("large", [7.5, 60.0, 700.0, 60000.0, 450000.0])
+@pytest.mark.parametrize("heavy", [True, False], ids=["heavy", "light"])
+def test_a_large_value_costs_the_other_groups_nothing(ctx, hd, large, heavy):
+    """The same with large numbers in the first group, of the heaviest tokens or of one
+    of the others.  With a scale below 2^(down + 1) the first group's products have 2^-down of
+    p's factor, 2^11, so that half of fp16's smallest number, 2^-25, times a
+    code of 8 is 2^(down - 33) of a token's term; p is 1 for one token of 32."""
+    n = 512
+    k, v = np.zeros((n, 1, hd), np.float32), np.ones((n, 1, hd), np.float32)
+    k[::2 * PAGE, 0, 0] = 17 * np.log(2) * np.sqrt(hd)
+    v[::2 * PAGE, 0] = 0
+    v[0 if heavy else 9::2 * PAGE, 0, 3] = large
+    kp, vp, k64, v64, table = one_sequence(np.random.default_rng(hd), k, v, n // PAGE)
+    q = np.zeros((1, hd))
+    q[0, 0] = 1
+    out, w = attend(ctx, q, kp, vp, table, n)
+    want, W, A, _ = attention(q, k64, v64)
+    assert (np.abs(want[:, 32:] * 2**12 - 1) < 0.05).all()
+    e = 6 * 2.0**-24 * 17 + 2.0**-19
+    tol = 2.0**-11 * np.abs(want) + (e + 2.0**-19) * A + n * 2.0**-33 + 2.0**-25
+    tol[:, :32] += 32 * 2.0**(np.floor(np.log2(large / 7)) + 1 - 33)
+    past = np.abs(want) >= 65520  # (fp16 has no such number)
+    assert (out[past] == np.inf).all()
+    off = np.where(past, 0, np.abs(np.where(past, 0, out) - want * ~past))
+    assert (off <= tol).all(), f"off by {(off / tol).max():.3g} of the bound"
+    assert (np.abs(w - W) <= (e + 2.0**-22) * W + 2.0**-40).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("order", [1, -1, 0], ids=["rising", "falling", "mixed"])
+def test_values_of_all_magnitudes(ctx, hd, order):
+    """Groups from 10^-3 to 10^4.6, in rising order, in falling and in none: a
+    wavefront makes room at many of its pairs.  Beside the roundings of
+    test_probabilities_keep_more_than_fp16 a token's term is off by 2^-34 of the
+    largest |V| of its group, whatever its weight, and by 2^-28 of its own |V|."""
+    rng = np.random.default_rng(hd + order)
+    n = 4000
+    mb = -(-n // PAGE)
+    size = rng.uniform(-3, 4.6, (n, 1, hd // 32))
+    size = size if order == 0 else np.sort(size, 0)[::order]
+    v = rng.uniform(-1, 1, (n, 1, hd)) * np.repeat(10.0**size, 32, -1)
+    kp, vp, k64, v64, table = one_sequence(rng, rng.normal(0, 1, (n, 1, hd)).astype(np.float32), v.astype(np.float32), mb)
+    q = np.zeros((8, hd))
+    q[np.arange(8), rng.integers(0, hd, 8)] = rng.choice([-2.0, -1.0, 1.0, 2.0], 8) * 8
+    out, w = attend(ctx, q, kp, vp, table, n)
+    want, W, A, _ = attention(q, k64, v64)
+    e = 6 * 2.0**-24 * np.abs(k64[:, 0] @ q.T).max() / np.sqrt(hd) + 2.0**-19
+    biggest = np.abs(v64[:, 0]).reshape(n, -1, 32).max((0, 2))  # of each group
+    tol = 2.0**-11 * np.abs(want) + (e + 2.0**-19) * A + 2.0**-25 + n * 2.0**-34 * np.repeat(biggest, 32) + 2.0**-28 * np.abs(v64[:, 0]).sum(0)
+    past = np.abs(want) >= 65520
+    assert not past.any()
+    off = np.abs(out - want)
+    assert (off <= tol).all(), f"off by {(off / tol).max():.3g} of the bound"
+    assert (np.abs(w - W) <= (e + 2.0**-21) * W + 2.0**-40).all()
+
+
 # ------------------------------------------------------------ shared buffers --
 @pytest.mark.parametrize("op", ["nx_kv_evict_f16", "nx_kv_evict_int4"])
 def test_eviction_refuses_pools_that_are_another_buffer(op):
