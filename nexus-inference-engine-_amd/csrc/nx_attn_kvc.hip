@@ -25,10 +25,10 @@
 // int4-g32: a step of 32 dimensions is one scale group, so codes enter the
 // products as exact fp16 integers and the scales stay outside: fp32 behind K's
 // product, in front of V's with the probability.  Between two bounds: vector
-// instructions beside the products (356 a pair of pages of 128 dimensions, 275
+// instructions beside the products (347 a pair of pages of 128 dimensions, 283
 // more a wavefront) take 57 % of the SIMDs' time, and a wavefront, which has half
-// a pair in flight, waits for memory in 48 % of its own: 32768 tokens of 8 kv heads
-// (38 MB) 12.6 us and a join of 3.9.
+// a pair in flight, waits for memory in 47 % of its own: 32768 tokens of 8 kv heads
+// (38 MB) 12.8 us and a join of 3.9.
 #include <algorithm>
 #include <type_traits>
 
